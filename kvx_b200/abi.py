@@ -107,10 +107,18 @@ class AttentionDesc(C.Structure):
                 ("block_table", BlockTable), ("seq_lens", SeqLens)]
 
 
+class ChunkAttentionDesc(C.Structure):
+    """``kvx_chunk_attention_desc_t`` (include/kvx_attention.h)."""
+    _fields_ = [("size", C.c_uint32), ("num_q_heads", C.c_uint32), ("max_seq_len", C.c_uint32),
+                ("scale", C.c_float), ("causal", C.c_uint32), ("query_indptr_dtype", C.c_int),
+                ("query", TensorDesc), ("out", TensorDesc), ("block_table", BlockTable),
+                ("seq_lens", SeqLens), ("query_indptr", C.c_void_p)]
+
+
 # x86-64 sizes frozen by the C header's static assertions.
 ABI_SIZES = {Version: 16, TensorDesc: 112, PoolDesc: 32, CacheDesc: 280, BlockTable: 64,
              SlotMapping: 32, SeqLens: 24, KvIoDesc: 248, ScaleDesc: 104, WriteDesc: 512,
-             GatherDesc: 352, AttentionDesc: 328}
+             GatherDesc: 352, AttentionDesc: 328, ChunkAttentionDesc: 344}
 for _cls, _bytes in ABI_SIZES.items():
     assert C.sizeof(_cls) == _bytes, (_cls.__name__, C.sizeof(_cls), _bytes)
 
@@ -268,4 +276,27 @@ def attention_desc(seq_count: int, q_heads: int, dim: int, io_dtype: int, query_
     b.indices_count = (seq_count * max_blocks_per_seq) & 0xFFFFFFFF
     a.seq_lens.size = C.sizeof(SeqLens)
     a.seq_lens.dtype, a.seq_lens.seq_count, a.seq_lens.lengths = index_dtype, seq_count, lens_addr
+    return a
+
+
+def chunk_attention_desc(seq_count: int, rows: int, q_heads: int, dim: int, io_dtype: int, query_addr: int, out_addr: int,
+                         scale: float, causal: bool, max_seq_len: int, index_dtype: int, table_addr: int,
+                         max_blocks_per_seq: int, lens_addr: int, indptr_dtype: int, indptr_addr: int,
+                         memory: int = MEMORY_DEVICE) -> ChunkAttentionDesc:
+    """A ``kvx_chunk_attention_desc_t`` with dense ``[rows, q_heads, dim]`` query / out and a PACKED
+    block table."""
+    a = ChunkAttentionDesc()
+    a.size = C.sizeof(ChunkAttentionDesc)
+    a.num_q_heads, a.max_seq_len, a.scale, a.causal = q_heads, max_seq_len, scale, int(causal)
+    a.query = tensor_desc(query_addr, io_dtype, (rows, q_heads, dim), memory=memory)
+    a.out = tensor_desc(out_addr, io_dtype, (rows, q_heads, dim), memory=memory)
+    b = a.block_table
+    b.size = C.sizeof(BlockTable)
+    b.format, b.index_dtype, b.seq_count, b.beam_width = TABLE_PACKED, index_dtype, seq_count, 1
+    b.max_blocks_per_seq = max_blocks_per_seq
+    b.indices = table_addr
+    b.indices_count = (seq_count * max_blocks_per_seq) & 0xFFFFFFFF
+    a.seq_lens.size = C.sizeof(SeqLens)
+    a.seq_lens.dtype, a.seq_lens.seq_count, a.seq_lens.lengths = index_dtype, seq_count, lens_addr
+    a.query_indptr_dtype, a.query_indptr = indptr_dtype, indptr_addr
     return a

@@ -1,0 +1,1895 @@
+/*
+ * Attention of a chunk of new tokens over the paged KV cache (include/kvx_attention.h): several
+ * query tokens per sequence -- a prompt, the next piece of one, drafted tokens to verify -- attend
+ * over the sequence's pages in place.  No reference counterpart; pages are found as the gather
+ * finds them (reference: kernels/kvx_paged_kv.cu:232-266, :54-75).
+ *
+ *   rows      The query heads of one KV head and the new tokens form the rows of one product: row
+ *             r = token * group + head of the group, so K and V are read once per KV head.
+ *   schedule  Tiles of rows, each with its causal number of K/V steps, are laid end to end and cut
+ *             into equal shares, one per CTA (a share may begin and end inside a tile).  Only the
+ *             tiles a cut goes through have partial results; the merge kernel joins them.
+ *   product   scores = Q K^T and out += P V on tcgen05.mma, accumulators in tensor memory, one pass
+ *             over K and V with the running maximum and sum of the softmax in f32.
+ *
+ * Nothing here allocates; plan and partial results live in caller-provided scratch.
+ */
+#include "kvx_attention.h"
+#include "kvx_paged_kv.h"
+
+#include "kvx_pages.h"
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <atomic>
+
+namespace {
+
+using kvx_detail::dtype_bytes;
+using kvx_detail::make_page_view;
+using kvx_detail::PageView;
+using kvx_detail::ScaleView;
+
+// ------------------------------------------------------------------ parameters ---------
+
+struct ChunkParams {
+  PageView k, v;
+  ScaleView ks, vs;
+  const void *table, *lens, *indptr;
+  const char *query;
+  char *out;
+  int64_t q_pitch, o_pitch;  // bytes between token rows
+  int64_t *prefix;           // [seq_count + 1] steps ahead of each sequence (all KV heads)
+  float *part_o;             // [2 * grid][slot_rows][dim] unnormalised sums of cut tiles
+  float *part_ml;            // [2 * grid][slot_rows][2] their maxima (unscaled scores) and denominators
+  float scale_log2;          // scale * log2(e)
+  int32_t seq_count, rows, max_blocks, max_seq_len, num_blocks, block_size;
+  int32_t heads_kv, group, dim;
+  int32_t causal, table64, indptr64;
+  int32_t cache_code, io_code;
+  int32_t grid, slot_rows, min_share;
+  int32_t tile_rows, kv_tile;  // rows and tokens of one step of this kernel
+  int32_t pair;                // 1: a tile of at most half the rows walks two K/V tiles per step
+  int32_t box;                 // tokens one TMA box loads
+  int32_t q_vec;               // 1: query rows can be read in 16-byte pieces
+  int32_t kv_vec;              // 1: page rows can be read in pieces of 8 elements
+};
+
+__device__ int g_chunk_error;  // set to 1 when a bounded wait gave up
+
+__device__ __forceinline__ int64_t read_index(const void *p, int64_t i, int wide) {
+  return wide ? static_cast<const int64_t *>(p)[i] : static_cast<const int32_t *>(p)[i];
+}
+
+__device__ __forceinline__ void pdl_prologue() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ------------------------------------------------------------------ schedule -----------
+
+// One sequence of the batch.  Row r of its group rows belongs to token r / group, whose position is
+// pos0 + token; it sees the cached tokens below limit(r).
+struct Seq {
+  int32_t first;  // first row of query / out
+  int32_t rows;   // new tokens * group
+  int32_t len;    // cached tokens that can take part
+  int32_t pos0;
+};
+
+__device__ __forceinline__ Seq load_seq(const ChunkParams &p, int s) {
+  const int64_t a = read_index(p.indptr, s, p.indptr64);
+  int64_t b = read_index(p.indptr, s + 1, p.indptr64);
+  if (b > p.rows) b = p.rows;
+  const int64_t n = (a < 0 || b <= a) ? 0 : b - a;
+  int64_t len = read_index(p.lens, s, p.table64);
+  if (len < 0) len = 0;
+  const int64_t pos0 = len - n;
+  len = min(len, static_cast<int64_t>(p.max_seq_len));
+  len = min(len, static_cast<int64_t>(p.max_blocks) * p.block_size);
+  Seq q;
+  q.first = n > 0 ? static_cast<int32_t>(a) : 0;
+  q.rows = static_cast<int32_t>(n * p.group);
+  q.len = static_cast<int32_t>(len);
+  q.pos0 = static_cast<int32_t>(min(pos0, len));  // at or beyond len every token sees all of it
+  return q;
+}
+
+__device__ __forceinline__ int32_t row_limit(const ChunkParams &p, const Seq &q, int32_t r) {
+  if (!p.causal) return q.len;
+  return max(0, min(q.len, q.pos0 + r / p.group + 1));
+}
+__device__ __forceinline__ int32_t tiles_of(const ChunkParams &p, const Seq &q) {
+  return (q.rows + p.tile_rows - 1) / p.tile_rows;
+}
+__device__ __forceinline__ bool is_narrow(const ChunkParams &p, const Seq &q) {
+  return p.pair != 0 && q.rows * 2 <= p.tile_rows;
+}
+// K/V tiles and steps of row tile `t`.  A tile without any is still one step: its rows are written.
+__device__ __forceinline__ int32_t kv_tiles_of(const ChunkParams &p, const Seq &q, int32_t t) {
+  const int32_t last = min(q.rows, (t + 1) * p.tile_rows) - 1;
+  return (row_limit(p, q, last) + p.kv_tile - 1) / p.kv_tile;
+}
+__device__ __forceinline__ int32_t steps_of(const ChunkParams &p, const Seq &q, int32_t t) {
+  int32_t n = kv_tiles_of(p, q, t);
+  if (is_narrow(p, q)) n = (n + 1) / 2;
+  return max(1, n);
+}
+
+constexpr int kPlanThreads = 1024;
+
+// prefix[s] = steps of the sequences ahead of s, over all KV heads.  One warp per sequence adds up
+// its tiles, then one scan over the warps' sums.
+__global__ void __launch_bounds__(kPlanThreads) kvx_chunk_plan_kernel(const ChunkParams p) {
+  pdl_prologue();
+  __shared__ int64_t s_sum[32];
+  __shared__ int64_t s_base;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) s_base = 0;
+  __syncthreads();
+  for (int s0 = 0; s0 < p.seq_count; s0 += kPlanThreads) {
+    // a thread adds up its own sequence when it has few tiles, a warp joins for the others
+    const int s = s0 + threadIdx.x;
+    Seq q{0, 0, 0, 0};
+    int32_t tiles = 0;
+    if (s < p.seq_count) {
+      q = load_seq(p, s);
+      tiles = tiles_of(p, q);
+    }
+    int64_t mine = 0;
+    if (tiles <= 8)
+      for (int t = 0; t < tiles; ++t) mine += steps_of(p, q, t);
+    unsigned big = __ballot_sync(0xFFFFFFFFu, tiles > 8);
+    while (big != 0) {
+      const int from = __ffs(big) - 1;
+      big &= big - 1;
+      Seq x;
+      x.first = 0;
+      x.rows = __shfl_sync(0xFFFFFFFFu, q.rows, from);
+      x.len = __shfl_sync(0xFFFFFFFFu, q.len, from);
+      x.pos0 = __shfl_sync(0xFFFFFFFFu, q.pos0, from);
+      const int32_t nt = tiles_of(p, x);
+      int64_t sum = 0;
+      for (int t = lane; t < nt; t += 32) sum += steps_of(p, x, t);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+      if (lane == from) mine = sum;
+    }
+    mine *= p.heads_kv;
+    int64_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    int64_t before = s_base;
+    for (int w = 0; w < warp; ++w) before += s_sum[w];
+    if (s < p.seq_count) p.prefix[s] = before + incl - mine;
+    __syncthreads();
+    if (threadIdx.x == kPlanThreads - 1) s_base = before + incl;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) p.prefix[p.seq_count] = s_base;
+}
+
+// A place in the laid-out work: step `off` of tile `tile` of KV head `head` of sequence `seq`.
+struct Place {
+  int32_t seq, head, tile, off;
+  int32_t steps;  // of the tile
+  Seq q;
+};
+
+__device__ __forceinline__ int shares(const ChunkParams &p, int64_t total) {
+  const int64_t want = (total + p.min_share - 1) / p.min_share;
+  return static_cast<int>(min(want, static_cast<int64_t>(p.grid)));
+}
+__device__ __forceinline__ int64_t share_begin(int64_t total, int n, int c) {
+  return total * c / n;  // total < 2^48, n < 2^15
+}
+
+// All lanes of a warp call it together and get the same answer.  `at` < prefix[seq_count].
+__device__ Place find_place(const ChunkParams &p, int64_t at) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.seq_count;  // the last s with prefix[s] <= at lies in [lo, hi)
+  while (hi - lo > 1) {
+    const int step = max(1, (hi - lo + 31) / 32);
+    const int s = lo + lane * step;
+    const unsigned in = __ballot_sync(0xFFFFFFFFu, s < hi && p.prefix[s] <= at);
+    lo = lo + (31 - __clz(in)) * step;
+    hi = min(hi, lo + step);
+  }
+  Place w;
+  w.seq = lo;
+  w.q = load_seq(p, lo);
+  const int64_t in_seq = at - p.prefix[lo];
+  const int64_t per_head = (p.prefix[lo + 1] - p.prefix[lo]) / p.heads_kv;
+  w.head = static_cast<int32_t>(in_seq / per_head);
+  int64_t left = in_seq - w.head * per_head;
+  const int32_t nt = tiles_of(p, w.q);
+  for (int t0 = 0;; t0 += 32) {
+    const int32_t n = t0 + lane < nt ? steps_of(p, w.q, t0 + lane) : 0;
+    int64_t incl = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    const unsigned beyond = __ballot_sync(0xFFFFFFFFu, incl > left);
+    if (beyond != 0) {
+      const int l = __ffs(beyond) - 1;
+      w.tile = t0 + l;
+      w.steps = __shfl_sync(0xFFFFFFFFu, n, l);
+      w.off = static_cast<int32_t>(left - (__shfl_sync(0xFFFFFFFFu, incl, l) - w.steps));
+      return w;
+    }
+    left -= __shfl_sync(0xFFFFFFFFu, incl, 31);
+    if (t0 + 32 >= nt) {  // not reached: `at` lies inside the sequence
+      w.tile = 0, w.off = 0, w.steps = 1;
+      return w;
+    }
+  }
+}
+
+// The next tile after w's, in the order of the schedule; w.seq = seq_count when there is none.
+__device__ __forceinline__ void next_tile(const ChunkParams &p, Place &w) {
+  w.off = 0;
+  if (++w.tile >= tiles_of(p, w.q)) {
+    w.tile = 0;
+    if (++w.head >= p.heads_kv) {
+      w.head = 0;
+      do {
+        if (++w.seq >= p.seq_count) return;
+        w.q = load_seq(p, w.seq);
+      } while (w.q.rows == 0);
+    }
+  }
+  w.steps = steps_of(p, w.q, w.tile);
+}
+
+// One CTA's part of one tile: steps [begin, end) of it.
+struct Piece {
+  Seq q;
+  int32_t seq, head, row0, rows;  // rows [row0, row0 + rows) of the sequence's group rows
+  int32_t kv0, kv1;               // K/V tiles of the piece
+  int32_t narrow;
+  int32_t slot;                   // partial-result slot, -1 = the piece is the whole tile
+};
+
+__device__ __forceinline__ Piece piece_of(const ChunkParams &p, const Place &w, int32_t end, int share) {
+  Piece x;
+  x.q = w.q;
+  x.seq = w.seq;
+  x.head = w.head;
+  x.row0 = w.tile * p.tile_rows;
+  x.rows = min(p.tile_rows, w.q.rows - x.row0);
+  x.narrow = is_narrow(p, w.q) ? 1 : 0;
+  const int32_t n = kv_tiles_of(p, w.q, w.tile);
+  const int32_t mul = x.narrow ? 2 : 1;
+  x.kv0 = min(n, w.off * mul);
+  x.kv1 = min(n, end * mul);
+  // a share holds at most one piece that continues a tile begun earlier and one that begins a
+  // tile ended later
+  x.slot = (w.off == 0 && end == w.steps) ? -1 : (w.off > 0 ? 2 * share : 2 * share + 1);
+  return x;
+}
+
+// ------------------------------------------------------------------ element access -----
+
+__device__ __forceinline__ float load_f32(const char *at, int code) {
+  switch (code) {
+    case KVX_DTYPE_BF16:
+      return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(at)) << 16);
+    case KVX_DTYPE_F16:
+      return __half2float(__ushort_as_half(*reinterpret_cast<const uint16_t *>(at)));
+    case KVX_DTYPE_F8_E4M3: {
+      uint32_t h2;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(*reinterpret_cast<const uint8_t *>(at))));
+      return __half2float(__ushort_as_half(static_cast<uint16_t>(h2 & 0xFFFFu)));
+    }
+    default:
+      return *reinterpret_cast<const float *>(at);
+  }
+}
+__device__ __forceinline__ void store_f32(char *base, int64_t i, float x, int code) {
+  if (code == KVX_DTYPE_BF16)
+    reinterpret_cast<uint16_t *>(base)[i] = __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  else if (code == KVX_DTYPE_F16)
+    reinterpret_cast<uint16_t *>(base)[i] = __half_as_ushort(__float2half_rn(x));
+  else
+    reinterpret_cast<float *>(base)[i] = x;
+}
+__device__ __forceinline__ int elem_bytes(int code) {
+  return code == KVX_DTYPE_F32 ? 4 : code == KVX_DTYPE_F8_E4M3 ? 1 : 2;
+}
+__device__ __forceinline__ int64_t head_offset(const PageView &v, int64_t o, int64_t h, int32_t d) {
+  const int32_t hi = d / v.pack;
+  return o * v.tok + h * v.head + hi * v.dhi + (d - hi * v.pack) * v.dlo;
+}
+
+// Page of token `tok` of sequence `seq`, -1 when it takes no part.
+__device__ __forceinline__ int32_t page_of(const ChunkParams &p, int32_t seq, int32_t tok) {
+  const int32_t lb = tok / p.block_size;
+  if (lb >= p.max_blocks) return -1;
+  const int64_t b = read_index(p.table, static_cast<int64_t>(seq) * p.max_blocks + lb, p.table64);
+  return b < 0 || b >= p.num_blocks ? -1 : static_cast<int32_t>(b);
+}
+
+// exp2 of a difference of scaled maxima, 0 when nothing was accumulated under `a`.
+__device__ __forceinline__ float weight_of(float a, float m, float mul) { return a == -INFINITY ? 0.f : exp2f((a - m) * mul); }
+
+// Score multiplier of a KV head in the exp2 domain (the K scale of an e4m3 cache folded in).
+__device__ __forceinline__ float score_mul(const ChunkParams &p, int head) {
+  return p.ks.base != nullptr ? p.scale_log2 * p.ks.base[head * p.ks.stride] : p.scale_log2;
+}
+
+// The kernels keep scores of a query whose sign makes the multiplier positive; a multiplier of zero
+// becomes a query of zeros (zero times the -inf of a masked score would be a NaN).
+__device__ __forceinline__ float score_abs(float mul) { return mul == 0.f ? 1.f : fabsf(mul); }
+
+// ------------------------------------------------------------------ merge of pieces ----
+
+constexpr int kMergeThreads = 128;
+
+// One warp per (cut, row of the tile the cut goes through); the first cut through a tile does the
+// work.
+__global__ void __launch_bounds__(kMergeThreads) kvx_chunk_merge_kernel(const ChunkParams p) {
+  pdl_prologue();
+  const int64_t total = p.prefix[p.seq_count];
+  const int n = shares(p, total);
+  const int cut = blockIdx.x + 1;
+  if (cut >= n) return;
+  const int64_t at = share_begin(total, n, cut);
+  const Place w = find_place(p, at);
+  if (w.off == 0) return;
+  const int64_t tile_at = at - w.off, tile_end = tile_at + w.steps;
+  if (share_begin(total, n, cut - 1) > tile_at) return;  // an earlier cut goes through this tile
+  // shares cut .. last continue the tile, share cut - 1 began it
+  int last = cut;
+  while (last + 1 < n && share_begin(total, n, last + 1) < tile_end) ++last;
+  const int32_t row0 = w.tile * p.tile_rows, rows = min(p.tile_rows, w.q.rows - row0);
+  const int lane = threadIdx.x & 31;
+  const float mul = score_abs(score_mul(p, w.head));
+  for (int r = blockIdx.y * (kMergeThreads / 32) + (threadIdx.x >> 5); r < rows; r += gridDim.y * (kMergeThreads / 32)) {
+    float m = -INFINITY;
+    for (int c = cut - 1 + lane; c <= last; c += 32) {
+      const int64_t slot = c == cut - 1 ? 2 * c + 1 : 2 * c;
+      m = fmaxf(m, p.part_ml[(slot * p.slot_rows + r) * 2]);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    float l = 0.f;
+    for (int c = cut - 1; c <= last; ++c) {
+      const int64_t slot = c == cut - 1 ? 2 * c + 1 : 2 * c;
+      const float2 ml = reinterpret_cast<const float2 *>(p.part_ml)[slot * p.slot_rows + r];
+      l += ml.y * weight_of(ml.x, m, mul);
+    }
+    const int32_t token = (row0 + r) / p.group, head = w.head * p.group + (row0 + r) % p.group;
+    char *out = p.out + (w.q.first + token) * p.o_pitch + static_cast<int64_t>(head) * p.dim * elem_bytes(p.io_code);
+    for (int d = lane; d < p.dim; d += 32) {
+      float acc = 0.f;
+      for (int c = cut - 1; c <= last; ++c) {
+        const int64_t slot = c == cut - 1 ? 2 * c + 1 : 2 * c;
+        const float f = weight_of(p.part_ml[(slot * p.slot_rows + r) * 2], m, mul);
+        acc += f * p.part_o[(slot * p.slot_rows + r) * p.dim + d];
+      }
+      store_f32(out, d, l == 0.f ? 0.f : acc / l, p.io_code);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ mbarriers, TMA, tensor memory --
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+
+// Waits for the phase; after two seconds, or when another warp gave up, sets the CTA's flag and
+// answers false, upon which every role returns.  (Inlined: a call here would have to save the
+// scores a softmax thread holds in registers.)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
+  if (mbar_try(bar, parity)) return true;
+  const uint64_t from = now_ns();
+#pragma unroll 1
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try(bar, parity)) return true;
+    if (*gave_up != 0) return false;
+    if (now_ns() - from > kWaitLimitNs) {
+      *gave_up = 1;
+      g_chunk_error = 1;
+      return false;
+    }
+  }
+}
+// The same for a whole warp: all lanes get one answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, gave_up)) != 0;
+}
+
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap *map, int x, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// d[128 x N] (+)= a[128 x 16] b[N x 16]^T; a and b in shared memory
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// the same with a in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tc_ld32(float *x, uint32_t at) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tc_ld16(uint32_t *r, uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Shared-memory operand descriptor, 128-byte swizzle: rows of 128 bytes, 8 of them to an atom of
+// 1 024 bytes.  `stride` bytes between groups of 8 rows; `lead` bytes between blocks of 64
+// elements along the rows (used when the rows run along the reduction, i.e. for V).
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
+         (static_cast<uint64_t>(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ float fast_exp2(float x) {  // ex2.approx: 2 ulp, -inf -> 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct Bf16 {
+  static constexpr uint32_t kFormat = 1;  // operand format of the instruction descriptor
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&r);
+  }
+  static __device__ __forceinline__ uint32_t from_f16x2(uint32_t x) {  // e4m3 values: exact
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+    return pack2(f.x, f.y);
+  }
+};
+struct Fp16 {
+  static constexpr uint32_t kFormat = 0;
+  static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 r = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&r);
+  }
+  static __device__ __forceinline__ uint32_t from_f16x2(uint32_t x) { return x; }
+};
+
+// ------------------------------------------------------------------ tensor-core kernel --
+//
+// Roles of a CTA (one per SM, 384 threads):
+//   warps 0-3, 4-7   softmax of stream 0 and of stream 1: a thread owns one of the 128 rows
+//   warp 8           one thread issues every tcgen05.mma
+//   warp 9           walks the schedule, publishes pieces, loads K and V tiles (TMA)
+//   warps 10, 11     help loading where pages cannot be read by TMA
+// Two streams of 128 rows keep the tensor pipe and the exponentials busy in turn: while one
+// stream's scores are turned into weights the other stream's products run.  A tile with at most
+// 128 rows gives both streams the same rows and every K/V tile to one of them; the two halves are
+// joined in shared memory.  head_dim above 128 leaves tensor memory for one stream, which then has
+// two score buffers instead.
+//
+// Tensor memory (512 columns): scores of 128 x 128 f32 at 0 and 128, weights written over the
+// first 64 columns of their scores, output sums at 256 (and 256 + kDp).  The MMAs of a CTA run in
+// the order of their issue, which is what lets the scores of the next tile overwrite the weights
+// the previous product read.
+
+constexpr int kThreads = 384;
+constexpr int kTile = 128;          // rows of a stream, tokens of a K/V tile
+constexpr int kPanelBytes = 16384;  // 128 rows x 128 bytes
+constexpr int kItems = 2;           // pieces published ahead
+
+template <int kDp>
+struct Shape {
+  static constexpr int kStreams = kDp > 128 ? 1 : 2;
+  static constexpr int kScoreBufs = kDp > 128 ? 2 : 1;     // per stream
+  static constexpr int kPanels = kDp / 64;                 // 64 dims (128 bytes) each
+  static constexpr int kUnitPanels = kPanels > 2 ? 2 : kPanels;
+  static constexpr int kUnits = kPanels / kUnitPanels;     // ring entries per K (or V) tile
+  static constexpr int kUnitBytes = kUnitPanels * kPanelBytes;
+  static constexpr int kStages = kDp == 64 ? 8 : 5;
+  static constexpr int kQBytes = kPanels * kPanelBytes;    // per stream
+  static constexpr int kRingAt = kStreams * kQBytes;
+  static constexpr int kMiscAt = kRingAt + kStages * kUnitBytes;
+};
+
+struct Misc {
+  uint64_t item_full[kItems], item_empty[kItems];
+  uint64_t kv_full[8], kv_empty[8];
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t tail, drain, join_full, join_empty;
+  Piece items[kItems];
+  float join_m[kTile], join_l[kTile];
+  uint32_t tmem;
+  int gave_up;
+};
+
+template <int kDp>
+constexpr size_t chunk_smem_bytes() {
+  return 1024 + Shape<kDp>::kMiscAt + sizeof(Misc);
+}
+
+// K/V tiles [b, e) stream `s` walks in this piece.
+template <int kStreams>
+__device__ __forceinline__ void stream_range(const ChunkParams &p, const Piece &x, int s, int *b, int *e) {
+  if (kStreams == 2 && x.narrow) {
+    const int h = x.kv0 + (x.kv1 - x.kv0 + 1) / 2;
+    *b = s == 0 ? x.kv0 : h;
+    *e = s == 0 ? h : x.kv1;
+    return;
+  }
+  const int rows = min(kTile, x.rows - s * kTile);
+  *b = *e = x.kv0;
+  if (rows <= 0) return;
+  const int32_t limit = row_limit(p, x.q, x.row0 + s * kTile + rows - 1);
+  *e = max(x.kv0, min(x.kv1, (limit + kTile - 1) / kTile));
+}
+
+// Loads the K and V tiles of a piece in the order in which Products::piece consumes them.
+template <int kStreams, typename Load>
+__device__ __forceinline__ bool walk_loads(const ChunkParams &p, const Piece &x, Load &&load) {
+  int b0, e0, b1 = 0, e1 = 0;
+  stream_range<kStreams>(p, x, 0, &b0, &e0);
+  if (kStreams == 2) stream_range<kStreams>(p, x, 1, &b1, &e1);
+  if (kStreams == 1) {
+    const int n = e0 - b0;
+    if (n > 0 && !load(false, b0)) return false;
+    for (int i = 0; i < n; ++i) {
+      if (i + 1 < n && !load(false, b0 + i + 1)) return false;
+      if (!load(true, b0 + i)) return false;
+    }
+    return true;
+  }
+  if (x.narrow) {
+    const int n0 = e0 - b0, n1 = e1 - b1;
+    if (n0 > 0 && !load(false, b0)) return false;
+    if (n1 > 0 && !load(false, b1)) return false;
+    for (int i = 0; i < n0; ++i) {
+      if (!load(true, b0 + i)) return false;
+      if (i + 1 < n0 && !load(false, b0 + i + 1)) return false;
+      if (i < n1 && !load(true, b1 + i)) return false;
+      if (i + 1 < n1 && !load(false, b1 + i + 1)) return false;
+    }
+    return true;
+  }
+  const int n = max(e0, e1) - x.kv0;
+  if (n > 0 && !load(false, x.kv0)) return false;
+  for (int i = 0; i < n; ++i) {
+    if (!load(true, x.kv0 + i)) return false;
+    if (i + 1 < n && !load(false, x.kv0 + i + 1)) return false;
+  }
+  return true;
+}
+
+struct Ring {
+  uint32_t stage = 0, phase = 0;
+  template <int kStages>
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) stage = 0, phase ^= 1;
+  }
+};
+
+// ---- loads ------------------------------------------------------------------------------
+
+template <int kDp>
+__device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, uint32_t base, Misc *m) {
+  using S = Shape<kDp>;
+  const int lane = threadIdx.x & 31;
+  volatile int *gave_up = &m->gave_up;
+  Ring ring;
+  uint32_t loads = 0;  // ring entries filled so far
+  uint32_t tail_phase = 0;
+  const int boxes = kTile / p.box;
+  const int64_t total = p.prefix[p.seq_count];
+  const int n = shares(p, total), share = blockIdx.x;
+  bool ok = true;
+  uint32_t item = 0;
+  if (share < n) {
+    int64_t at = share_begin(total, n, share);
+    const int64_t end = share_begin(total, n, share + 1);
+    Place w = find_place(p, at);
+    while (ok && at < end) {
+      const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + (end - at)));
+      const Piece x = piece_of(p, w, stop, share);
+      const uint32_t slot = item % kItems;
+      if (item >= kItems) ok = warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up);
+      if (!ok) break;
+      if (lane == 0) {
+        m->items[slot] = x;
+        mbar_arrive(smem_addr(&m->item_full[slot]));
+      }
+      ++item;
+      ok = walk_loads<S::kStreams>(p, x, [&](bool is_v, int tile) {
+        // every lane < boxes owns one box: its page, or (beyond the sequence, no such page) a page
+        // number behind the pool, which TMA answers with zeros
+        int32_t page = p.num_blocks, in_page = 0;
+        if (lane < boxes) {
+          const int32_t tok = tile * kTile + lane * p.box;
+          if (tok < x.q.len) {
+            const int32_t b = page_of(p, x.seq, tok);
+            if (b >= 0) page = b, in_page = tok % p.block_size;
+          }
+        }
+        const int valid = x.q.len - tile * kTile;  // tokens of the tile that exist
+        const bool tail = is_v && valid < kTile && valid % p.box != 0;
+        const bool head_inner = p.k.head < p.k.tok;  // order of the map's middle dimensions
+        for (int u = 0; u < S::kUnits; ++u) {
+          const uint32_t st = ring.stage;
+          if (loads >= S::kStages && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase ^ 1, gave_up)) return false;
+          const uint32_t dst = base + S::kRingAt + st * S::kUnitBytes;
+          const uint32_t bar = smem_addr(tail ? &m->tail : &m->kv_full[st]);
+          if (lane == 0) mbar_expect_tx(bar, S::kUnitBytes);
+          __syncwarp();
+          if (lane < boxes) {
+            for (int pp = 0; pp < S::kUnitPanels; ++pp) {
+              const int x0 = (u * S::kUnitPanels + pp) * 64;
+              tma_load4(dst + pp * kPanelBytes + lane * p.box * 128, is_v ? vmap : kmap, x0, head_inner ? x.head : in_page,
+                        head_inner ? in_page : x.head, page, bar);
+            }
+          }
+          if (tail) {
+            // Rows of the last page behind the sequence hold whatever the page holds; their weight
+            // is zero, but zero times a NaN is not: overwrite them.
+            if (!warp_wait(bar, tail_phase, gave_up)) return false;
+            tail_phase ^= 1;
+            const int upto = min(kTile, (valid + p.box - 1) / p.box * p.box);
+            for (int i = lane; i < (upto - valid) * 8 * S::kUnitPanels; i += 32) {
+              const int pp = i / ((upto - valid) * 8), j = i - pp * (upto - valid) * 8;
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + pp * kPanelBytes + valid * 128 + j * 16), "r"(0u)
+                           : "memory");
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&m->kv_full[st]));
+          }
+          ring.next<S::kStages>();
+          ++loads;
+        }
+        return true;
+      });
+      at += stop - w.off;
+      if (at < end) next_tile(p, w);
+    }
+  }
+  if (ok) {
+    const uint32_t slot = item % kItems;
+    if (item >= kItems) ok = warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up);
+    if (ok && lane == 0) {
+      m->items[slot].rows = 0;  // no more pieces
+      mbar_arrive(smem_addr(&m->item_full[slot]));
+    }
+  }
+  // Nothing may be in flight towards this CTA's shared memory when it ends.  Normally: every
+  // entry's release has arrived.  After giving up: the loads themselves, as far as they come.
+  const uint32_t held = min(loads, static_cast<uint32_t>(S::kStages));
+  for (uint32_t k = 0; k < held; ++k) {
+    const uint32_t entry = loads - held + k, st = entry % S::kStages, ph = (entry / S::kStages) & 1;
+    if (ok) ok = warp_wait(smem_addr(&m->kv_empty[st]), ph, gave_up);
+    if (!ok) {
+      int ignore = 0;
+      for (int i = 0; i < 4096 && ignore == 0; ++i) ignore = mbar_try(smem_addr(&m->kv_full[st]), ph) ? 1 : 0;
+    }
+  }
+}
+
+// Pages that TMA cannot read (e4m3, HND_PACKED, odd page sizes, odd strides): three warps copy rows
+// into the same swizzled tiles, converting on the way.  Warp 9 walks the schedule here, too.
+template <typename T, int kDp>
+__device__ void load_role_copy(const ChunkParams &p, uint32_t base, Misc *m) {
+  using S = Shape<kDp>;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - 9, tid = threadIdx.x - 9 * 32;
+  volatile int *gave_up = &m->gave_up;
+  Ring ring;
+  uint32_t loads = 0, item = 0;
+  const int64_t total = p.prefix[p.seq_count];
+  const int n = shares(p, total), share = blockIdx.x;
+  int64_t at = 0, end = 0;
+  Place w;
+  if (share < n) {
+    at = share_begin(total, n, share);
+    end = share_begin(total, n, share + 1);
+    w = find_place(p, at);
+  }
+  const int elem = elem_bytes(p.cache_code);
+  while (at < end) {
+    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + (end - at)));
+    const Piece x = piece_of(p, w, stop, share);
+    if (warp == 0) {
+      const uint32_t slot = item % kItems;
+      if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up)) return;
+      if (lane == 0) {
+        m->items[slot] = x;
+        mbar_arrive(smem_addr(&m->item_full[slot]));
+      }
+    }
+    ++item;
+    const bool ok = walk_loads<S::kStreams>(p, x, [&](bool is_v, int tile) {
+      const PageView &view = is_v ? p.v : p.k;
+      for (int u = 0; u < S::kUnits; ++u) {
+        const uint32_t st = ring.stage;
+        if (loads >= S::kStages && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase ^ 1, gave_up)) return false;
+        const uint32_t dst = base + S::kRingAt + st * S::kUnitBytes;
+        constexpr int kChunks = S::kUnitPanels * 8;  // 16-byte pieces of a row in this unit
+        constexpr int kBatch = 4;
+        for (int i0 = tid; i0 < kTile * kChunks; i0 += 96 * kBatch) {
+          uint4 r[kBatch];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + 96 * k;
+            r[k] = make_uint4(0, 0, 0, 0);
+            if (i >= kTile * kChunks) continue;
+            const int row = i / kChunks, d = u * S::kUnitPanels * 64 + (i % kChunks) * 8;
+            const int32_t tok = tile * kTile + row;
+            if (tok >= x.q.len || d >= p.dim) continue;
+            const int32_t page = page_of(p, x.seq, tok);
+            if (page < 0) continue;
+            const char *from = view.base + page * view.blk;
+            const int32_t o = tok % p.block_size;
+            if (p.kv_vec) {
+              const char *src = from + o * view.tok + x.head * view.head + static_cast<int64_t>(d) * elem;
+              if (elem == 2)
+                r[k] = *reinterpret_cast<const uint4 *>(src);
+              else
+                *reinterpret_cast<uint2 *>(&r[k]) = *reinterpret_cast<const uint2 *>(src);
+            } else {
+              uint16_t e[8];
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                e[c] = 0;
+                if (d + c < p.dim) {
+                  const char *src = from + head_offset(view, o, x.head, d + c);
+                  e[c] = elem == 2 ? *reinterpret_cast<const uint16_t *>(src) : *reinterpret_cast<const uint8_t *>(src);
+                }
+              }
+              if (elem == 2)
+                r[k] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+              else
+                r[k] = make_uint4(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const int i = i0 + 96 * k;
+            if (i >= kTile * kChunks) continue;
+            uint4 y = r[k];
+            if (elem == 1) {
+              uint32_t h[4];
+              asm("{ .reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b; }"
+                  : "=r"(h[0]), "=r"(h[1]) : "r"(r[k].x));
+              asm("{ .reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b; }"
+                  : "=r"(h[2]), "=r"(h[3]) : "r"(r[k].y));
+              y = make_uint4(T::from_f16x2(h[0]), T::from_f16x2(h[1]), T::from_f16x2(h[2]), T::from_f16x2(h[3]));
+            }
+            const int row = i / kChunks, c = i % kChunks;
+            const uint32_t to = dst + (c >> 3) * kPanelBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&m->kv_full[st]));
+        ring.next<S::kStages>();
+        ++loads;
+      }
+      return true;
+    });
+    if (!ok) return;
+    at += stop - w.off;
+    if (at < end) next_tile(p, w);
+  }
+  if (warp == 0) {
+    const uint32_t slot = item % kItems;
+    if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up)) return;
+    if (lane == 0) {
+      m->items[slot].rows = 0;
+      mbar_arrive(smem_addr(&m->item_full[slot]));
+    }
+  }
+  const uint32_t held = min(loads, static_cast<uint32_t>(S::kStages));  // releases that are still to arrive
+  for (uint32_t k = 0; k < held; ++k) {
+    const uint32_t entry = loads - held + k;
+    if (!warp_wait(smem_addr(&m->kv_empty[entry % S::kStages]), (entry / S::kStages) & 1, gave_up)) return;
+  }
+}
+
+// ---- products -----------------------------------------------------------------------------
+
+template <typename T, int kDp>
+struct Products {
+  using S = Shape<kDp>;
+  // instruction descriptors: f32 accumulator, M = 128, B K-major (scores) or N-major (output)
+  static constexpr uint32_t kTypes = (1u << 4) | (T::kFormat << 7) | (T::kFormat << 10) | ((kTile >> 4) << 24);
+  static constexpr uint32_t kScores = kTypes | ((kTile >> 3) << 17);
+  static constexpr uint32_t kOutput = kTypes | (1u << 16) | ((S::kUnitPanels * 64 / 8) << 17);
+
+  uint32_t base, tmem;
+  Misc *m;
+  volatile int *gave_up;
+  Ring ring;
+  uint32_t tiles[2] = {0, 0};   // score tiles issued per stream
+  uint32_t weights[2] = {0, 0};  // output products issued per stream
+
+  __device__ __forceinline__ bool acquire(Ring *first) {  // one K or V tile
+    *first = ring;
+    for (int u = 0; u < S::kUnits; ++u) {
+      if (!mbar_wait(smem_addr(&m->kv_full[ring.stage]), ring.phase, gave_up)) return false;
+      ring.next<S::kStages>();
+    }
+    return true;
+  }
+  __device__ __forceinline__ void release(Ring from) {
+    for (int u = 0; u < S::kUnits; ++u) {
+      tc_commit(smem_addr(&m->kv_empty[from.stage]));
+      from.next<S::kStages>();
+    }
+  }
+  __device__ __forceinline__ void scores(int s, Ring k) {
+    tc_fence_after();
+    const uint32_t buf = S::kScoreBufs == 2 ? (tiles[s] & 1) : s;
+    const uint32_t d = tmem + buf * kTile;
+    const uint32_t q = base + s * S::kQBytes;
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u) {
+      const uint32_t at = base + S::kRingAt + k.stage * S::kUnitBytes;
+#pragma unroll
+      for (int kk = 0; kk < S::kUnitPanels * 4; ++kk) {
+        const uint32_t in = (kk >> 2) * kPanelBytes + (kk & 3) * 32;
+        mma_ss(d, operand_desc(q + u * S::kUnitPanels * kPanelBytes + in, 16, 1024), operand_desc(at + in, 16, 1024), kScores,
+               u > 0 || kk > 0);
+      }
+      k.next<S::kStages>();
+    }
+    tc_commit(smem_addr(&m->s_full[buf]));
+    ++tiles[s];
+  }
+  __device__ __forceinline__ bool wait_weights(int s) {
+    const uint32_t buf = S::kScoreBufs == 2 ? (weights[s] & 1) : s;
+    const uint32_t ph = (S::kScoreBufs == 2 ? weights[s] >> 1 : weights[s]) & 1;
+    return mbar_wait(smem_addr(&m->p_full[buf]), ph, gave_up);
+  }
+  __device__ __forceinline__ void output(int s, Ring v, bool first) {
+    tc_fence_after();
+    const uint32_t buf = S::kScoreBufs == 2 ? (weights[s] & 1) : s;
+    const uint32_t a = tmem + buf * kTile, d = tmem + 256 + s * kDp;
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u) {
+      const uint32_t at = base + S::kRingAt + v.stage * S::kUnitBytes;
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; ++kk)
+        mma_ts(d + u * 128, a + kk * 8, operand_desc(at + kk * 2048, kPanelBytes, 1024), kOutput, !first || kk > 0);
+      v.next<S::kStages>();
+    }
+    tc_commit(smem_addr(&m->pv_done[s]));
+    ++weights[s];
+  }
+
+  __device__ bool piece(const ChunkParams &p, const Piece &x, uint32_t *queries) {
+    int b[2] = {0, 0}, e[2] = {0, 0};
+    for (int s = 0; s < S::kStreams; ++s) {
+      stream_range<S::kStreams>(p, x, s, &b[s], &e[s]);
+      if (e[s] > b[s] && !mbar_wait(smem_addr(&m->q_full[s]), queries[s]++ & 1, gave_up)) return false;
+    }
+    const int n0 = e[0] - b[0], n1 = e[1] - b[1];
+    Ring k, v;
+    if (S::kStreams == 1) {
+      if (n0 > 0) {
+        if (!acquire(&k)) return false;
+        scores(0, k);
+        release(k);
+      }
+      for (int i = 0; i < n0; ++i) {
+        if (i + 1 < n0) {
+          if (!acquire(&k)) return false;
+          scores(0, k);
+          release(k);
+        }
+        if (!wait_weights(0) || !acquire(&v)) return false;
+        output(0, v, i == 0);
+        release(v);
+      }
+      return true;
+    }
+    if (x.narrow) {
+      for (int s = 0; s < 2; ++s) {
+        if (e[s] == b[s]) continue;
+        if (!acquire(&k)) return false;
+        scores(s, k);
+        release(k);
+      }
+      for (int i = 0; i < n0; ++i) {
+        for (int s = 0; s < 2; ++s) {
+          const int n = s == 0 ? n0 : n1;
+          if (i >= n) continue;
+          if (!wait_weights(s) || !acquire(&v)) return false;
+          output(s, v, i == 0);
+          release(v);
+          if (i + 1 < n) {
+            if (!acquire(&k)) return false;
+            scores(s, k);
+            release(k);
+          }
+        }
+      }
+      return true;
+    }
+    const int n = max(n0, n1);
+    if (n > 0) {
+      if (!acquire(&k)) return false;
+      if (n0 > 0) scores(0, k);
+      if (n1 > 0) scores(1, k);
+      release(k);
+    }
+    for (int i = 0; i < n; ++i) {
+      if (i < n0 && !wait_weights(0)) return false;
+      if (!acquire(&v)) return false;
+      if (i < n0) output(0, v, i == 0);
+      if (i + 1 < n) {
+        if (!acquire(&k)) return false;
+        if (i + 1 < n0) scores(0, k);
+      }
+      if (i < n1) {
+        if (!wait_weights(1)) return false;
+        output(1, v, i == 0);
+      }
+      release(v);
+      if (i + 1 < n) {
+        if (i + 1 < n1) scores(1, k);
+        release(k);
+      }
+    }
+    return true;
+  }
+};
+
+// ---- softmax ------------------------------------------------------------------------------
+
+// Raises the weights' reference maximum only when it has moved by more than this (in the exp2
+// domain): weights then stay below 2^8, the rounding of a weight is relative either way, and the
+// sums in tensor memory are rescaled on a few tiles instead of on every one.
+constexpr float kLazy = 8.f;
+
+// One row of a piece again, token by token and only those it may see.  A masked token has weight
+// zero in the products, but zero times an infinity or a NaN that its V holds is a NaN: a row that
+// comes out of the products not finite although tokens were masked for it is redone here.
+template <int kDp>
+__device__ void redo_row(const ChunkParams &p, const Piece &x, int32_t r, float mul, float *o, float *m_out, float *l_out) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kPer = kDp / 32;
+  const int32_t token = r / p.group, qh = x.head * p.group + r % p.group;
+  const char *q = p.query + (x.q.first + token) * p.q_pitch + static_cast<int64_t>(qh) * p.dim * 2;
+  float qv[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int d = lane + 32 * i;
+    qv[i] = d < p.dim ? load_f32(q + d * 2, p.io_code) : 0.f;
+    if (mul < 0.f) qv[i] = -qv[i];
+    if (mul == 0.f) qv[i] = 0.f;
+    o[i] = 0.f;
+  }
+  const float am = score_abs(mul);
+  float m = -INFINITY, l = 0.f;
+  const int32_t end = min(row_limit(p, x.q, r), x.kv1 * kTile);
+  for (int32_t t = x.kv0 * kTile; t < end; ++t) {
+    const int32_t page = page_of(p, x.seq, t);
+    if (page < 0) continue;
+    const int32_t at = t % p.block_size;
+    const char *kp = p.k.base + page * p.k.blk, *vp = p.v.base + page * p.v.blk;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int d = lane + 32 * i;
+      if (d < p.dim) dot = fmaf(qv[i], load_f32(kp + head_offset(p.k, at, x.head, d), p.cache_code), dot);
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, s);
+    const float mn = fmaxf(m, dot);
+    const float c = weight_of(m, mn, am);
+    const float w = mn == -INFINITY ? (dot == dot ? 0.f : dot) : exp2f((dot - mn) * am);
+    l = l * c + w;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int d = lane + 32 * i;
+      const float vv = d < p.dim ? load_f32(vp + head_offset(p.v, at, x.head, d), p.cache_code) : 0.f;
+      o[i] = o[i] * c + (w == 0.f ? 0.f * vv : w * vv);
+    }
+    m = mn;
+  }
+  *m_out = m, *l_out = l;
+}
+
+template <typename T, int kDp>
+__device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, uint32_t tmem0, Misc *m) {
+  using S = Shape<kDp>;
+  const int s = threadIdx.x >> 7;                 // stream
+  const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
+  const uint32_t lanes = static_cast<uint32_t>((tid >> 5) * 32) << 16;  // this warp's lanes of tensor memory
+  volatile int *gave_up = &m->gave_up;
+  uint32_t tiles = 0;       // score tiles of this stream so far
+  uint32_t joins = 0;
+  for (uint32_t item = 0;; ++item) {
+    const uint32_t slot = item % kItems;
+    if (!warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1, gave_up)) return;
+    const Piece x = m->items[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_addr(&m->item_empty[slot]));
+    if (x.rows == 0) return;
+    int b, e;
+    stream_range<S::kStreams>(p, x, s, &b, &e);
+    const bool narrow = S::kStreams == 2 && x.narrow;
+    const int32_t row_at = x.row0 + (narrow ? 0 : s * kTile);   // first group row of this stream
+    const int32_t rows = min(kTile, x.rows - (narrow ? 0 : s * kTile));
+    if (rows <= 0) continue;
+    const float mul = score_mul(p, x.head);
+    const float am = score_abs(mul);
+
+    if (e > b) {
+      // Query rows into the swizzled operand tile (its last reader, the scores of this stream's
+      // previous tile, was waited for).
+      const uint32_t flip = mul < 0.f ? 0x80008000u : 0u, keep = mul == 0.f ? 0u : 0xFFFFFFFFu;
+      constexpr int kChunks = kDp / 8;
+      for (int i = tid; i < kTile * kChunks; i += 128) {
+        const int row = i / kChunks, c = i % kChunks, d = c * 8;
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (row < rows && d < p.dim) {
+          const int32_t r = row_at + row, token = r / p.group, h = x.head * p.group + (r - token * p.group);
+          const char *src = p.query + (x.q.first + token) * p.q_pitch + (static_cast<int64_t>(h) * p.dim + d) * 2;
+          if (p.q_vec) {
+            y = *reinterpret_cast<const uint4 *>(src);
+          } else {
+            uint16_t t[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = d + k < p.dim ? reinterpret_cast<const uint16_t *>(src)[k] : 0;
+            y = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+          }
+          y.x = (y.x ^ flip) & keep, y.y = (y.y ^ flip) & keep, y.z = (y.z ^ flip) & keep, y.w = (y.w ^ flip) & keep;
+        }
+        const uint32_t to = base + s * S::kQBytes + (c >> 3) * kPanelBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&m->q_full[s]));
+    }
+
+    // (rows behind the tile's last are never written: nothing is masked for them)
+    const int32_t limit = tid < rows ? row_limit(p, x.q, row_at + tid) : INT32_MAX;
+    float mx = -INFINITY, l = 0.f;
+    const uint32_t o_at = tmem0 + lanes + 256 + s * kDp;
+    for (int j = b; j < e; ++j, ++tiles) {
+      const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
+      const uint32_t ph = (S::kScoreBufs == 2 ? tiles >> 1 : tiles) & 1;
+      const uint32_t s_at = tmem0 + lanes + buf * kTile;
+      // does every page of the tile exist?  four tokens per lane (page sizes that are not a
+      // multiple of four are looked up token by token below)
+      int32_t page_ok = 1;
+      {
+        const int32_t tok = j * kTile + lane * 4;
+        if (tok < x.q.len) page_ok = (p.block_size & 3) == 0 && page_of(p, x.seq, tok) >= 0;
+      }
+      const int32_t valid = limit == INT32_MAX ? kTile : min(kTile, limit - j * kTile);  // visible tokens of this row (may be negative)
+      const bool masked = __any_sync(0xFFFFFFFFu, valid < kTile) != 0;
+      const bool holes = __all_sync(0xFFFFFFFFu, page_ok) == 0;
+      if (!warp_wait(smem_addr(&m->s_full[buf]), ph, gave_up)) return;
+      tc_fence_after();
+      float sc[kTile];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tc_ld32(sc + 32 * c, s_at + 32 * c);
+      tc_wait_ld();
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < kTile; ++c)
+          if (c >= valid) sc[c] = -INFINITY;
+      }
+      if (holes) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int32_t tok = j * kTile + c * 32 + lane;
+          const unsigned has = __ballot_sync(0xFFFFFFFFu, tok >= x.q.len || page_of(p, x.seq, tok) >= 0);
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (!((has >> k) & 1)) sc[32 * c + k] = -INFINITY;
+        }
+      }
+      float t0 = fmaxf(sc[0], sc[1]), t1 = fmaxf(sc[2], sc[3]);
+#pragma unroll
+      for (int c = 4; c < kTile; c += 4) {
+        t0 = fmaxf(fmaxf(t0, sc[c]), sc[c + 1]);
+        t1 = fmaxf(fmaxf(t1, sc[c + 2]), sc[c + 3]);
+      }
+      const float top = fmaxf(t0, t1);
+      const bool raise = top > mx && (mx == -INFINITY || (top - mx) * am > kLazy);
+      if (__any_sync(0xFFFFFFFFu, raise)) {
+        const float c = raise ? weight_of(mx, top, am) : 1.f;
+        if (raise) mx = top;
+        if (j > b) {
+          l *= c;
+          // the sums of the tiles so far must be complete before they are rescaled
+          if (!warp_wait(smem_addr(&m->pv_done[s]), (tiles - 1) & 1, gave_up)) return;
+          tc_fence_after();
+#pragma unroll 1
+          for (int k = 0; k < kDp / 16; ++k) {
+            uint32_t o[16];
+            tc_ld16(o, o_at + 16 * k);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+            tc_st16(o_at + 16 * k, o);
+          }
+        }
+      }
+      // weights exp2((score - mx) * am); a row that has seen no token yet subtracts 0
+      const float sub = mx == -INFINITY ? 0.f : -mx * am;
+      const float2 am2 = make_float2(am, am), sub2 = make_float2(sub, sub);
+      float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float2 z = __ffma2_rn(make_float2(sc[32 * c + 2 * k], sc[32 * c + 2 * k + 1]), am2, sub2);
+          const float2 y = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+          sum2 = __fadd2_rn(sum2, y);
+          w[k] = T::pack2(y.x, y.y);
+        }
+        tc_st16(s_at + 16 * c, w);
+      }
+      l += sum2.x + sum2.y;
+      tc_wait_st();
+      // One stream: the scores of this tile were issued ahead of the previous output product, so they
+      // do not tell that it has ended.  Weights are handed over only after it has -- the barrier is
+      // then never more than one phase away from the parity that is waited for.
+      if (S::kScoreBufs == 2 && j > b && !warp_wait(smem_addr(&m->pv_done[s]), (tiles - 1) & 1, gave_up)) return;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&m->p_full[buf]));
+    }
+
+    if (e > b) {
+      if (!warp_wait(smem_addr(&m->pv_done[s]), (tiles - 1) & 1, gave_up)) return;
+      tc_fence_after();
+    }
+    // ---- the piece's result ----
+    const float vmul = p.vs.base != nullptr ? p.vs.base[x.head * p.vs.stride] : 1.f;
+    float f_own = 1.f, f_other = 0.f;
+    const bool join = narrow && x.kv1 - x.kv0 > 1;  // stream 1 has tiles of its own
+    if (join) {
+      if (s == 1) {
+        // hand sums, maximum and denominator to stream 0 through this stream's query tile
+        m->join_m[tid] = mx, m->join_l[tid] = l;
+        float *buf = reinterpret_cast<float *>(smem + S::kQBytes);  // [kDp / 2][128]
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (half == 1) {
+            if (!warp_wait(smem_addr(&m->join_empty), joins & 1, gave_up)) return;
+            ++joins;
+          }
+#pragma unroll
+          for (int k = 0; k < kDp / 64; ++k) {
+            float o[32];
+            tc_ld32(o, o_at + half * (kDp / 2) + 32 * k);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) buf[(32 * k + i) * kTile + tid] = o[i];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&m->join_full));
+        }
+        // the query tile is free again once stream 0 has read the second half
+        if (!warp_wait(smem_addr(&m->join_empty), joins & 1, gave_up)) return;
+        ++joins;
+        tc_fence_before();
+        continue;
+      }
+    } else if (narrow && s == 1) {
+      continue;
+    }
+    uint32_t join_at = joins;
+    if (join) {
+      if (!warp_wait(smem_addr(&m->join_full), join_at & 1, gave_up)) return;
+      const float m1 = m->join_m[tid], l1 = m->join_l[tid];
+      const float top = fmaxf(mx, m1);
+      f_own = weight_of(mx, top, am), f_other = weight_of(m1, top, am);
+      l = l * f_own + l1 * f_other;
+      mx = top;
+    }
+    const int32_t r = row_at + tid;
+    const int32_t token = r / p.group, qh = x.head * p.group + r % p.group;
+    const float *joined = reinterpret_cast<const float *>(smem + S::kQBytes);
+    char *out = p.out + (x.q.first + token) * p.o_pitch + static_cast<int64_t>(qh) * p.dim * 2;
+    const int64_t part = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + (r - x.row0);
+    const float mul_out = l == 0.f ? 0.f : (x.slot < 0 ? vmul / l : vmul);
+    float finite = 0.f;
+    const bool vec_out = p.q_vec != 0;
+#pragma unroll
+    for (int k = 0; k < kDp / 32; ++k) {
+      if (join && k == kDp / 64) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&m->join_empty));
+        if (!warp_wait(smem_addr(&m->join_full), (join_at + 1) & 1, gave_up)) return;
+      }
+      float o[32];
+      if (e > b) {
+        tc_ld32(o, o_at + 32 * k);
+        tc_wait_ld();
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float y = e > b ? o[i] : 0.f;
+        if (join) y = y * f_own + joined[((k % (kDp / 64)) * 32 + i) * kTile + tid] * f_other;
+        y *= mul_out;
+        if (l == 0.f) y = 0.f;
+        finite = fmaf(y, 0.f, finite);  // NaN as soon as one value is not finite
+        o[i] = y;
+      }
+      if (tid < rows) {
+        if (x.slot >= 0) {
+          float *to = p.part_o + part * p.dim + 32 * k;
+          if ((p.dim & 3) == 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (32 * k + i < p.dim) *reinterpret_cast<float4 *>(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * k + i < p.dim) to[i] = o[i];
+          }
+        } else if (vec_out) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (32 * k + i < p.dim)
+              *reinterpret_cast<uint4 *>(out + (32 * k + i) * 2) =
+                  make_uint4(T::pack2(o[i], o[i + 1]), T::pack2(o[i + 2], o[i + 3]), T::pack2(o[i + 4], o[i + 5]), T::pack2(o[i + 6], o[i + 7]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * k + i < p.dim) store_f32(out, 32 * k + i, o[i], p.io_code);
+        }
+      }
+    }
+    if (join) {
+      joins += 2;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&m->join_empty));
+    }
+    if (x.slot >= 0 && tid < rows) reinterpret_cast<float2 *>(p.part_ml)[part] = make_float2(mx, l);
+    tc_fence_before();
+    const int32_t seen = min(x.q.len, x.kv1 * kTile);
+    unsigned again = __ballot_sync(0xFFFFFFFFu, tid < rows && finite != 0.f && limit < seen);
+    while (again != 0) {
+      const int from = __ffs(again) - 1;
+      again &= again - 1;
+      const int32_t rr = row_at + (tid & ~31) + from;
+      float o[kDp / 32], m2, l2;
+      redo_row<kDp>(p, x, rr, mul, o, &m2, &l2);
+      const float f = l2 == 0.f ? 0.f : (x.slot < 0 ? vmul / l2 : vmul);
+      const int32_t tk = rr / p.group, hh = x.head * p.group + rr % p.group;
+      char *to = p.out + (x.q.first + tk) * p.o_pitch + static_cast<int64_t>(hh) * p.dim * 2;
+      const int64_t slot_row = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + (rr - x.row0);
+#pragma unroll
+      for (int i = 0; i < kDp / 32; ++i) {
+        const int d = lane + 32 * i;
+        if (d >= p.dim) continue;
+        const float y = l2 == 0.f ? 0.f : o[i] * f;
+        if (x.slot >= 0)
+          p.part_o[slot_row * p.dim + d] = y;
+        else
+          store_f32(to, d, y, p.io_code);
+      }
+      if (x.slot >= 0 && lane == 0) reinterpret_cast<float2 *>(p.part_ml)[slot_row] = make_float2(m2, l2);
+    }
+  }
+}
+
+template <typename T, int kDp, bool kTma>
+__global__ void __launch_bounds__(kThreads, 1)
+    kvx_chunk_attention_kernel(const ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using S = Shape<kDp>;
+  extern __shared__ char smem_raw[];
+  char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t base = smem_addr(smem);
+  Misc *m = reinterpret_cast<Misc *>(smem + S::kMiscAt);
+  const int warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(smem_addr(&m->item_full[i]), 1);
+      mbar_init(smem_addr(&m->item_empty[i]), S::kStreams * 4 + 1);  // softmax warps and the issuing thread
+    }
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(smem_addr(&m->kv_full[i]), kTma ? 1 : 3);
+      mbar_init(smem_addr(&m->kv_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&m->q_full[i]), 4);
+      mbar_init(smem_addr(&m->s_full[i]), 1);
+      mbar_init(smem_addr(&m->p_full[i]), 4);
+      mbar_init(smem_addr(&m->pv_done[i]), 1);
+    }
+    mbar_init(smem_addr(&m->tail), 1);
+    mbar_init(smem_addr(&m->drain), 1);
+    mbar_init(smem_addr(&m->join_full), 4);
+    mbar_init(smem_addr(&m->join_empty), 4);
+    m->gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&m->tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = m->tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if ((warp >> 2) < S::kStreams) softmax_role<T, kDp>(p, base, smem, tmem, m);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      if ((threadIdx.x & 31) == 0) {
+        Products<T, kDp> pr;
+        pr.base = base, pr.tmem = tmem, pr.m = m, pr.gave_up = &m->gave_up;
+        uint32_t queries[2] = {0, 0};
+        for (uint32_t item = 0;; ++item) {
+          const uint32_t slot = item % kItems;
+          if (!mbar_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1, &m->gave_up)) break;
+          const Piece x = m->items[slot];
+          mbar_arrive(smem_addr(&m->item_empty[slot]));
+          if (x.rows == 0 || !pr.piece(p, x, queries)) break;
+        }
+        // every product has ended before tensor memory is given back
+        tc_commit(smem_addr(&m->drain));
+        int never = 0;
+        mbar_wait(smem_addr(&m->drain), 0, &never);
+      }
+      __syncwarp();
+    } else if (kTma) {
+      if (warp == 9) load_role_tma<kDp>(p, &kmap, &vmap, base, m);
+    } else {
+      load_role_copy<T, kDp>(p, base, m);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// ------------------------------------------------------------------ f32 and everything else --
+//
+// f32 caches (and queries), head_dim above 256: the same schedule and the same one-pass softmax on
+// the f32 units.  A step is 32 rows x kN tokens: scores from shared memory, a warp owns 4 rows of
+// the softmax and of the output sums (a lane owns every 32nd dim), K and V share one buffer.
+
+constexpr int kSimtThreads = 256;
+constexpr int kSimtRows = 32;
+constexpr int simt_tokens(int dim_bucket) { return dim_bucket > 512 ? 16 : 32; }
+
+template <int kDb>  // head_dim rounded up to 64, 128, 256, 512 or 1024
+__global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(const ChunkParams p) {
+  constexpr int kN = kDb > 512 ? 16 : 32;  // = simt_tokens(kDb)
+  constexpr int kPer = kDb / 32;
+  extern __shared__ float sm[];
+  const int dp = (p.dim + 3) & ~3, pitch = dp + 4;
+  float *sm_q = sm;                          // [32][pitch]
+  float *sm_kv = sm_q + kSimtRows * pitch;   // [kN][pitch]
+  float *sm_p = sm_kv + kN * pitch;          // [32][kN + 4]
+  int32_t *sm_page = reinterpret_cast<int32_t *>(sm_p + kSimtRows * (kN + 4));  // [kN]
+  pdl_prologue();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t total = p.prefix[p.seq_count];
+  const int n = shares(p, total), share = blockIdx.x;
+  if (share >= n) return;
+  int64_t at = share_begin(total, n, share);
+  const int64_t end = share_begin(total, n, share + 1);
+  Place w = find_place(p, at);
+  const int io = elem_bytes(p.io_code);
+  while (at < end) {
+    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + (end - at)));
+    const Piece x = piece_of(p, w, stop, share);
+    const float mul = score_mul(p, x.head), am = score_abs(mul);
+    __syncthreads();  // the previous piece is done with shared memory
+    for (int i = tid; i < kSimtRows * dp; i += kSimtThreads) {
+      const int row = i / dp, d = i - row * dp;
+      float y = 0.f;
+      if (row < x.rows && d < p.dim) {
+        const int32_t r = x.row0 + row, token = r / p.group, h = x.head * p.group + (r - token * p.group);
+        y = load_f32(p.query + (x.q.first + token) * p.q_pitch + (static_cast<int64_t>(h) * p.dim + d) * io, p.io_code);
+      }
+      sm_q[row * pitch + d] = mul < 0.f ? -y : mul == 0.f ? 0.f : y;
+    }
+    float acc[4][kPer], m[4], l[4];
+    int32_t limit[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = -INFINITY, l[i] = 0.f;
+      limit[i] = warp * 4 + i < x.rows ? row_limit(p, x.q, x.row0 + warp * 4 + i) : 0;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[i][k] = 0.f;
+    }
+    for (int j = x.kv0; j < x.kv1; ++j) {
+      const int32_t t0 = j * kN;
+      if (tid < kN) sm_page[tid] = t0 + tid < x.q.len ? page_of(p, x.seq, t0 + tid) : -1;
+      __syncthreads();  // pages known, query in place; the previous step is done with K/V and weights
+      for (int i = tid; i < kN * dp; i += kSimtThreads) {
+        const int c = i / dp, d = i - c * dp;
+        const int32_t page = sm_page[c];
+        float y = 0.f;
+        if (page >= 0 && d < p.dim)
+          y = load_f32(p.k.base + page * p.k.blk + head_offset(p.k, (t0 + c) % p.block_size, x.head, d), p.cache_code);
+        sm_kv[c * pitch + d] = y;
+      }
+      __syncthreads();
+      {
+        constexpr int kC = kN / 16;
+        const int ty = tid >> 4, tx = tid & 15;
+        float s[2][kC];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int b = 0; b < kC; ++b) s[a][b] = 0.f;
+        for (int d = 0; d < dp; d += 4) {
+          float4 q[2], k[kC];
+#pragma unroll
+          for (int a = 0; a < 2; ++a) q[a] = *reinterpret_cast<const float4 *>(&sm_q[(ty + 16 * a) * pitch + d]);
+#pragma unroll
+          for (int b = 0; b < kC; ++b) k[b] = *reinterpret_cast<const float4 *>(&sm_kv[(tx + 16 * b) * pitch + d]);
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < kC; ++b)
+              s[a][b] = fmaf(q[a].w, k[b].w, fmaf(q[a].z, k[b].z, fmaf(q[a].y, k[b].y, fmaf(q[a].x, k[b].x, s[a][b]))));
+        }
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int b = 0; b < kC; ++b) sm_p[(ty + 16 * a) * (kN + 4) + tx + 16 * b] = s[a][b];
+      }
+      __syncthreads();  // scores in place, K no longer needed
+      for (int i = tid; i < kN * dp; i += kSimtThreads) {
+        const int c = i / dp, d = i - c * dp;
+        const int32_t page = sm_page[c];
+        float y = 0.f;
+        if (page >= 0 && d < p.dim)
+          y = load_f32(p.v.base + page * p.v.blk + head_offset(p.v, (t0 + c) % p.block_size, x.head, d), p.cache_code);
+        sm_kv[c * pitch + d] = y;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a warp's own rows: no barrier between scores and weights
+        const int row = warp * 4 + i;
+        const bool in = lane < kN && t0 + lane < limit[i] && sm_page[lane < kN ? lane : 0] >= 0;
+        const float s = in ? sm_p[row * (kN + 4) + lane] : -INFINITY;
+        float top = s;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        const float mn = fmaxf(m[i], top);
+        const float c = weight_of(m[i], mn, am);
+        float wgt = 0.f;
+        if (in) wgt = mn == -INFINITY ? (s == s ? 0.f : s) : exp2f((s - mn) * am);
+        float sum = wgt;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        l[i] = l[i] * c + sum;
+        m[i] = mn;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[i][k] *= c;
+        if (lane < kN) sm_p[row * (kN + 4) + lane] = wgt;
+      }
+      __syncthreads();  // V in place, weights in place
+#pragma unroll
+      for (int c0 = 0; c0 < kN; c0 += 4) {
+        float4 wv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) wv[i] = *reinterpret_cast<const float4 *>(&sm_p[(warp * 4 + i) * (kN + 4) + c0]);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int d = lane + 32 * k;
+          if (d >= p.dim) continue;
+          float v[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = sm_kv[(c0 + c) * pitch + d];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (t0 + c0 + 3 < limit[i]) {
+              acc[i][k] = fmaf(wv[i].w, v[3], fmaf(wv[i].z, v[2], fmaf(wv[i].y, v[1], fmaf(wv[i].x, v[0], acc[i][k]))));
+            } else {  // tokens this row may not see are left out, not weighted with zero
+              if (t0 + c0 < limit[i]) acc[i][k] = fmaf(wv[i].x, v[0], acc[i][k]);
+              if (t0 + c0 + 1 < limit[i]) acc[i][k] = fmaf(wv[i].y, v[1], acc[i][k]);
+              if (t0 + c0 + 2 < limit[i]) acc[i][k] = fmaf(wv[i].z, v[2], acc[i][k]);
+            }
+          }
+        }
+      }
+    }
+    const float vmul = p.vs.base != nullptr ? p.vs.base[x.head * p.vs.stride] : 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = warp * 4 + i;
+      if (row >= x.rows) continue;
+      const int32_t r = x.row0 + row, token = r / p.group, qh = x.head * p.group + r % p.group;
+      char *out = p.out + (x.q.first + token) * p.o_pitch + static_cast<int64_t>(qh) * p.dim * io;
+      const int64_t part = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + row;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int d = lane + 32 * k;
+        if (d >= p.dim) continue;
+        if (x.slot >= 0)
+          p.part_o[part * p.dim + d] = acc[i][k] * vmul;
+        else
+          store_f32(out, d, l[i] == 0.f ? 0.f : acc[i][k] / l[i] * vmul, p.io_code);
+      }
+      if (x.slot >= 0 && lane == 0) reinterpret_cast<float2 *>(p.part_ml)[part] = make_float2(m[i], l[i]);
+    }
+    at += stop - w.off;
+    if (at < end) next_tile(p, w);
+  }
+}
+
+// ------------------------------------------------------------------ host ---------------
+
+constexpr int kMaxShares = 148;      // of the tensor-core kernel: one CTA per SM
+constexpr int kMaxSimtShares = 296;  // of the f32 kernel
+constexpr int kMinShare = 2;         // steps; a shorter share costs more in its partial result than it saves
+constexpr int kMinSimtShare = 4;
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Split {
+  int32_t tile_rows, kv_tile, grid, slot_rows, min_share;
+  size_t prefix_bytes, ml_bytes, o_bytes;
+  size_t total() const { return prefix_bytes + ml_bytes + o_bytes; }
+};
+
+// Scratch and shares of one kernel family.  Every share that begins or ends inside a tile has a
+// slot for it; there are never more shares than steps / min_share.
+Split split_of(bool tensor, int64_t seqs, int64_t rows, int64_t heads_q, int64_t heads_kv, int64_t dim, int64_t max_len) {
+  Split s;
+  const int64_t group = heads_q / heads_kv;
+  s.tile_rows = tensor ? (dim > 128 ? kTile : 2 * kTile) : kSimtRows;
+  s.kv_tile = tensor ? kTile : simt_tokens(static_cast<int>(dim > 512 ? 1024 : 64));
+  s.min_share = tensor ? kMinShare : kMinSimtShare;
+  const int64_t most = tensor ? kMaxShares : (dim > 256 ? kMaxShares : kMaxSimtShares);
+  const int64_t tiles = (seqs + rows * group / s.tile_rows) * heads_kv;
+  const int64_t per_tile = std::max<int64_t>(1, (max_len + s.kv_tile - 1) / s.kv_tile);
+  int64_t steps;
+  if (__builtin_mul_overflow(tiles, per_tile, &steps)) steps = INT64_MAX / 2;
+  s.grid = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(most, (steps + s.min_share - 1) / s.min_share)));
+  s.slot_rows = static_cast<int32_t>(std::min<int64_t>(s.tile_rows, rows * group));
+  s.prefix_bytes = (static_cast<size_t>(seqs + 1) * sizeof(int64_t) + 15) / 16 * 16;
+  const size_t slots = s.grid > 1 ? static_cast<size_t>(2) * s.grid * s.slot_rows : 0;
+  s.ml_bytes = slots * 2 * sizeof(float);
+  s.o_bytes = slots * dim * sizeof(float);
+  return s;
+}
+
+// Token rows of heads x dim elements without gaps, further apart than that or not.
+kvx_status_t check_rows(const kvx_tensor_desc_t *t, int64_t rows, int64_t heads, int64_t dim) {
+  if (t->size < sizeof(kvx_tensor_desc_t)) return KVX_STATUS_INVALID_ARGUMENT;
+  if (t->ndim != 3 || t->shape[0] != rows || t->shape[1] != heads || t->shape[2] != dim) return KVX_STATUS_INVALID_ARGUMENT;
+  if ((dim > 1 && t->stride[2] != 1) || (heads > 1 && t->stride[1] != dim)) return KVX_STATUS_UNSUPPORTED;
+  if (rows > 1 && t->stride[0] < heads * dim) return KVX_STATUS_UNSUPPORTED;
+  return KVX_STATUS_OK;
+}
+
+// Launch with the programmatic-stream-serialization attribute (see pdl_prologue).
+template <typename... Args>
+void launch_pdl(void (*kernel)(Args...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+EncodeTiled encode_tiled() {
+  static std::atomic<void *> cached{nullptr};
+  void *f = cached.load(std::memory_order_acquire);
+  if (f == nullptr) {
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    cached.store(f, std::memory_order_release);
+  }
+  return reinterpret_cast<EncodeTiled>(f);
+}
+
+// Pages as a 4-d tensor (dim, head and token in the order of their strides, page) loaded in boxes
+// of 64 dims x `box` tokens of one head of one page, swizzled as the operands want them.
+bool make_map(CUtensorMap *map, const ChunkParams &p, const PageView &v, bool bf16) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const bool head_inner = p.k.head < p.k.tok;
+  const cuuint64_t heads = static_cast<cuuint64_t>(p.heads_kv), toks = static_cast<cuuint64_t>(p.block_size);
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.dim), head_inner ? heads : toks, head_inner ? toks : heads,
+                              static_cast<cuuint64_t>(p.num_blocks)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(head_inner ? v.head : v.tok), static_cast<cuuint64_t>(head_inner ? v.tok : v.head),
+                                 static_cast<cuuint64_t>(v.blk)};
+  const cuuint32_t rows = static_cast<cuuint32_t>(p.box);
+  const cuuint32_t box[4] = {64, head_inner ? 1 : rows, head_inner ? rows : 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, v.base, dims, strides, box, step,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tma_strides(const PageView &v) {
+  const int64_t most = int64_t{1} << 40;
+  return v.pack == 1 && v.dhi == 2 && aligned16(v.base) && v.blk % 16 == 0 && v.tok % 16 == 0 && v.head % 16 == 0 && v.blk > 0 &&
+         v.tok > 0 && v.head > 0 && v.blk < most && v.tok < most && v.head < most;
+}
+
+template <typename T, int kDp, bool kTma>
+void launch_tensor(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t st) {
+  const size_t smem = chunk_smem_bytes<kDp>();
+  // (the attribute is per device and cheap to set, so it is set on every launch)
+  cudaFuncSetAttribute(kvx_chunk_attention_kernel<T, kDp, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_pdl(kvx_chunk_attention_kernel<T, kDp, kTma>, dim3(static_cast<unsigned>(p.grid)), kThreads, smem, st, p, k, v);
+}
+template <typename T, bool kTma>
+void launch_tensor_dim(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t st) {
+  if (p.dim <= 64)
+    launch_tensor<T, 64, kTma>(p, k, v, st);
+  else if (p.dim <= 128)
+    launch_tensor<T, 128, kTma>(p, k, v, st);
+  else
+    launch_tensor<T, 256, kTma>(p, k, v, st);
+}
+template <int kDb>
+void launch_simt(const ChunkParams &p, cudaStream_t st) {
+  const int pitch = ((p.dim + 3) & ~3) + 4, tokens = simt_tokens(kDb);
+  const size_t smem = static_cast<size_t>((kSimtRows + tokens) * pitch + kSimtRows * (tokens + 4) + tokens) * sizeof(float);
+  cudaFuncSetAttribute(kvx_chunk_attention_simt_kernel<kDb>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_pdl(kvx_chunk_attention_simt_kernel<kDb>, dim3(static_cast<unsigned>(p.grid)), kSimtThreads, smem, st, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+KVX_API size_t kvx_paged_attention_chunk_workspace_bytes(uint32_t seq_count, uint32_t num_rows, uint32_t num_q_heads,
+                                                         uint32_t num_kv_heads, uint32_t head_dim, uint32_t max_seq_len) {
+  if (seq_count == 0 || num_rows == 0 || num_q_heads == 0 || num_kv_heads == 0 || num_q_heads < num_kv_heads || head_dim == 0) return 0;
+  const Split a = split_of(true, seq_count, num_rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
+  const Split b = split_of(false, seq_count, num_rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
+  return std::max(a.total(), b.total());
+}
+
+KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *cache, const kvx_chunk_attention_desc_t *attn,
+                                                      const kvx_scale_desc_t *k_scale, const kvx_scale_desc_t *v_scale,
+                                                      void *workspace, size_t workspace_bytes, void *stream) {
+  if (cache == nullptr || attn == nullptr) return KVX_STATUS_INVALID_ARGUMENT;
+  if (cache->size < sizeof(kvx_cache_desc_t) || attn->size < sizeof(kvx_chunk_attention_desc_t) ||
+      attn->block_table.size < sizeof(kvx_block_table_t) || attn->seq_lens.size < sizeof(kvx_seq_lens_t))
+    return KVX_STATUS_INVALID_ARGUMENT;
+  const int64_t H = cache->num_kv_heads, D = cache->head_dim, Hq = attn->num_q_heads;
+  if (H == 0 || D == 0 || Hq == 0 || Hq % H != 0 || cache->block_size == 0 || attn->max_seq_len == 0)
+    return KVX_STATUS_INVALID_ARGUMENT;
+  if (cache->k.dtype != cache->v.dtype || attn->causal > 1) return KVX_STATUS_INVALID_ARGUMENT;
+  if (attn->block_table.format != KVX_BLOCK_TABLE_PACKED) return KVX_STATUS_UNSUPPORTED;
+  const kvx_dtype_t io = attn->query.dtype, cd = cache->k.dtype;
+  if ((io != KVX_DTYPE_F16 && io != KVX_DTYPE_BF16 && io != KVX_DTYPE_F32) || attn->out.dtype != io) return KVX_STATUS_UNSUPPORTED;
+  ChunkParams p = {};
+  if (cd == KVX_DTYPE_F8_E4M3) {
+    if (!kvx_detail::resolve_scale(k_scale, nullptr, cache->num_kv_heads, &p.ks) ||
+        !kvx_detail::resolve_scale(v_scale, nullptr, cache->num_kv_heads, &p.vs))
+      return KVX_STATUS_UNSUPPORTED;
+  } else if (cd != io) {
+    return KVX_STATUS_UNSUPPORTED;
+  }
+  const int64_t S = attn->block_table.seq_count, R = attn->query.shape[0];
+  if (attn->seq_lens.seq_count != S || R < 0) return KVX_STATUS_INVALID_ARGUMENT;
+  kvx_status_t st = check_rows(&attn->query, R, Hq, D);
+  if (st != KVX_STATUS_OK) return st;
+  st = check_rows(&attn->out, R, Hq, D);
+  if (st != KVX_STATUS_OK) return st;
+  const bool s32 = attn->block_table.index_dtype == KVX_DTYPE_S32 && attn->seq_lens.dtype == KVX_DTYPE_S32;
+  const bool s64 = attn->block_table.index_dtype == KVX_DTYPE_S64 && attn->seq_lens.dtype == KVX_DTYPE_S64;
+  if (!s32 && !s64) return KVX_STATUS_INVALID_ARGUMENT;
+  if (attn->query_indptr_dtype != KVX_DTYPE_S32 && attn->query_indptr_dtype != KVX_DTYPE_S64) return KVX_STATUS_INVALID_ARGUMENT;
+  if (S == 0 || R == 0) return KVX_STATUS_OK;
+  const int64_t elem = dtype_bytes(cd), io_elem = dtype_bytes(io);
+  st = make_page_view(cache, &cache->k, elem, &p.k);
+  if (st != KVX_STATUS_OK) return st;
+  st = make_page_view(cache, &cache->v, elem, &p.v);
+  if (st != KVX_STATUS_OK) return st;
+  if (attn->query.data == nullptr || attn->out.data == nullptr || attn->query_indptr == nullptr ||
+      attn->block_table.indices == nullptr || attn->seq_lens.lengths == nullptr || cache->k.data == nullptr ||
+      cache->v.data == nullptr || attn->block_table.max_blocks_per_seq == 0 ||
+      attn->block_table.max_blocks_per_seq > static_cast<uint32_t>(INT32_MAX) || cache->num_blocks > static_cast<uint32_t>(INT32_MAX) ||
+      cache->block_size > static_cast<uint32_t>(INT32_MAX) || attn->max_seq_len > static_cast<uint32_t>(INT32_MAX) - 1024u ||
+      S > INT32_MAX || D > INT32_MAX)
+    return KVX_STATUS_INVALID_ARGUMENT;
+  const int64_t group = Hq / H;
+  if (R > (INT32_MAX - 1024) / group) return KVX_STATUS_UNSUPPORTED;  // group rows are counted in 32 bits
+
+  const bool tensor = io != KVX_DTYPE_F32 && D <= 256;
+  if (!tensor && D > 1024) return KVX_STATUS_UNSUPPORTED;
+  const Split sp = split_of(tensor, S, R, Hq, H, D, attn->max_seq_len);
+  const size_t need = kvx_paged_attention_chunk_workspace_bytes(static_cast<uint32_t>(S), static_cast<uint32_t>(R), attn->num_q_heads,
+                                                                cache->num_kv_heads, cache->head_dim, attn->max_seq_len);
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) return KVX_STATUS_INVALID_ARGUMENT;
+
+  p.table = attn->block_table.indices;
+  p.lens = attn->seq_lens.lengths;
+  p.indptr = attn->query_indptr;
+  p.query = static_cast<const char *>(attn->query.data);
+  p.out = static_cast<char *>(attn->out.data);
+  p.q_pitch = (R > 1 ? attn->query.stride[0] : Hq * D) * io_elem;
+  p.o_pitch = (R > 1 ? attn->out.stride[0] : Hq * D) * io_elem;
+  p.prefix = static_cast<int64_t *>(workspace);
+  p.part_ml = reinterpret_cast<float *>(static_cast<char *>(workspace) + sp.prefix_bytes);
+  p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + sp.prefix_bytes + sp.ml_bytes);
+  p.scale_log2 = attn->scale * 1.4426950408889634f;
+  p.seq_count = static_cast<int32_t>(S);
+  p.rows = static_cast<int32_t>(R);
+  p.max_blocks = static_cast<int32_t>(attn->block_table.max_blocks_per_seq);
+  p.max_seq_len = static_cast<int32_t>(attn->max_seq_len);
+  p.num_blocks = static_cast<int32_t>(cache->num_blocks);
+  p.block_size = static_cast<int32_t>(cache->block_size);
+  p.heads_kv = static_cast<int32_t>(H);
+  p.group = static_cast<int32_t>(group);
+  p.dim = static_cast<int32_t>(D);
+  p.causal = static_cast<int32_t>(attn->causal);
+  p.table64 = s64 ? 1 : 0;
+  p.indptr64 = attn->query_indptr_dtype == KVX_DTYPE_S64 ? 1 : 0;
+  p.cache_code = static_cast<int32_t>(cd);
+  p.io_code = static_cast<int32_t>(io);
+  p.grid = sp.grid;
+  p.slot_rows = sp.slot_rows;
+  p.min_share = sp.min_share;
+  p.tile_rows = sp.tile_rows;
+  p.kv_tile = sp.kv_tile;
+  p.pair = tensor && D <= 128 ? 1 : 0;
+  p.q_vec = D % 8 == 0 && p.q_pitch % 16 == 0 && p.o_pitch % 16 == 0 && aligned16(p.query) && aligned16(p.out) ? 1 : 0;
+  const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+
+  launch_pdl(kvx_chunk_plan_kernel, dim3(1), static_cast<unsigned>(kPlanThreads), size_t{0}, cs, p);
+  if (tensor) {
+    p.box = 1;
+    while (p.box < kTile && p.block_size % (2 * p.box) == 0) p.box *= 2;
+    if (H == 1) {  // a stride nothing is multiplied by
+      if (p.k.head <= 0 || p.k.head % 16 != 0) p.k.head = p.k.tok;
+      if (p.v.head <= 0 || p.v.head % 16 != 0) p.v.head = p.v.tok;
+    }
+    CUtensorMap kmap = {}, vmap = {};
+    bool tma = elem == 2 && p.box >= 8 && tma_strides(p.k) && tma_strides(p.v) && (p.k.head < p.k.tok) == (p.v.head < p.v.tok);
+    tma = tma && make_map(&kmap, p, p.k, io == KVX_DTYPE_BF16) && make_map(&vmap, p, p.v, io == KVX_DTYPE_BF16);
+    const int64_t piece = 8 * elem;  // bytes one lane copies at a time where TMA is not used
+    auto rows_ok = [&](const PageView &v) {
+      return v.pack == 1 && v.dhi == elem && reinterpret_cast<uintptr_t>(v.base) % piece == 0 && v.blk % piece == 0 && v.tok % piece == 0 &&
+             v.head % piece == 0;
+    };
+    p.kv_vec = D % 8 == 0 && rows_ok(p.k) && rows_ok(p.v) ? 1 : 0;
+    if (io == KVX_DTYPE_BF16) {
+      if (tma)
+        launch_tensor_dim<Bf16, true>(p, kmap, vmap, cs);
+      else
+        launch_tensor_dim<Bf16, false>(p, kmap, vmap, cs);
+    } else {
+      if (tma)
+        launch_tensor_dim<Fp16, true>(p, kmap, vmap, cs);
+      else
+        launch_tensor_dim<Fp16, false>(p, kmap, vmap, cs);
+    }
+  } else if (D <= 64) {
+    launch_simt<64>(p, cs);
+  } else if (D <= 128) {
+    launch_simt<128>(p, cs);
+  } else if (D <= 256) {
+    launch_simt<256>(p, cs);
+  } else if (D <= 512) {
+    launch_simt<512>(p, cs);
+  } else {
+    launch_simt<1024>(p, cs);
+  }
+  if (p.grid > 1) {
+    const unsigned y = static_cast<unsigned>(std::max(1, std::min(16, p.slot_rows / 16)));
+    launch_pdl(kvx_chunk_merge_kernel, dim3(static_cast<unsigned>(p.grid - 1), y), static_cast<unsigned>(kMergeThreads), size_t{0}, cs, p);
+  }
+  return cudaGetLastError() == cudaSuccess ? KVX_STATUS_OK : KVX_STATUS_INTERNAL_ERROR;
+}
+
+KVX_API int kvx_attention_device_error(int reset) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_chunk_error, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (reset && v != 0) {
+    const int zero = 0;
+    if (cudaMemcpyToSymbol(g_chunk_error, &zero, sizeof(zero)) != cudaSuccess) cudaGetLastError();
+  }
+  return v != 0 ? 1 : 0;
+}
+
+}  // extern "C"

@@ -329,6 +329,73 @@ def paged_attention_decode(query: torch.Tensor, key_cache: torch.Tensor, value_c
     return out
 
 
+def paged_attention_chunk(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                          block_table: torch.Tensor, seq_lens: torch.Tensor, query_indptr: torch.Tensor,
+                          scale: float, causal: bool = True, max_seq_len: Optional[int] = None,
+                          out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                          kv_cache_dtype: str = "auto", k_scale: Optional[torch.Tensor] = None,
+                          v_scale: Optional[torch.Tensor] = None,
+                          num_kv_heads: Optional[int] = None) -> torch.Tensor:
+    """Attention of several new tokens per sequence over the paged cache
+    (``include/kvx_attention.h``): row ``query_indptr[s] + i`` of ``query`` ``[rows, q_heads, dim]``
+    is new token ``i`` of sequence ``s`` at position ``seq_lens[s] - n + i`` (``n`` new tokens, whose
+    K and V are in the pages already) and attends to the cached tokens up to its own position, or
+    to all of them when not ``causal``.  Returns ``out`` (same shape and dtype); rows of no sequence
+    keep what ``out`` held.  Token rows of ``query`` and ``out`` may be slices of wider rows.
+    ``workspace`` is reusable uint8 scratch of :func:`chunk_attention_workspace_bytes` bytes,
+    allocated per call when not given; ``max_seq_len`` and ``num_kv_heads`` as in
+    :func:`paged_attention_decode`."""
+    if query.dim() != 3 or query.dtype not in _FLOAT_CODES:
+        raise ValueError("query must be a [rows, q_heads, dim] float tensor")
+    if block_table.dim() != 2 or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous [seq_count, max_blocks_per_seq] tensor")
+    if block_table.dtype not in _INDEX_CODES or seq_lens.dtype != block_table.dtype:
+        raise TypeError("block_table and seq_lens must share an int32 or int64 dtype")
+    seqs = block_table.shape[0]
+    if seq_lens.dim() != 1 or seq_lens.numel() != seqs or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous with one entry per row of block_table")
+    if query_indptr.dtype not in _INDEX_CODES or query_indptr.dim() != 1 or query_indptr.numel() != seqs + 1 \
+            or not query_indptr.is_contiguous():
+        raise ValueError("query_indptr must hold seq_count + 1 int32 or int64 row numbers")
+    rows, q_heads, dim = query.shape
+    if out is None:
+        out = torch.empty((rows, q_heads, dim), dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype:
+        raise ValueError("out must have the shape and dtype of query")
+    for name, t in (("key_cache", key_cache), ("value_cache", value_cache), ("block_table", block_table),
+                    ("seq_lens", seq_lens), ("query_indptr", query_indptr), ("out", out)):
+        if not t.is_cuda or t.device != query.device:
+            raise ValueError(f"{name} must be on the query's CUDA device")
+    cache = cache_desc_from_tensors(key_cache, value_cache, kv_cache_dtype, num_kv_heads)
+    if cache.head_dim != dim:
+        raise ValueError("query and cache differ in head_dim")
+    if max_seq_len is None:
+        max_seq_len = min(block_table.shape[1] * cache.block_size, 2 ** 31 - 2048)
+    need = chunk_attention_workspace_bytes(seqs, rows, q_heads, cache.num_kv_heads, dim, max_seq_len)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=query.device)
+    a = abi.chunk_attention_desc(seqs, rows, q_heads, dim, _FLOAT_CODES[query.dtype], query.data_ptr(), out.data_ptr(),
+                                 float(scale), causal, int(max_seq_len), _INDEX_CODES[block_table.dtype],
+                                 block_table.data_ptr(), block_table.shape[1], seq_lens.data_ptr(),
+                                 _INDEX_CODES[query_indptr.dtype], query_indptr.data_ptr())
+    for t, src in ((a.query, query), (a.out, out)):
+        for i, s in enumerate(src.stride()):
+            t.stride[i] = s
+    ks, vs = _scale_desc(k_scale, cache.num_kv_heads), _scale_desc(v_scale, cache.num_kv_heads)
+    with torch.cuda.device(query.device):
+        status = lib().kvx_launch_paged_attention_chunk(
+            C.byref(cache), C.byref(a), C.byref(ks), C.byref(vs), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx chunk attention", status)
+    return out
+
+
+def chunk_attention_workspace_bytes(seq_count: int, rows: int, q_heads: int, kv_heads: int, dim: int,
+                                    max_seq_len: int) -> int:
+    return lib().kvx_paged_attention_chunk_workspace_bytes(seq_count, rows, q_heads, kv_heads, dim, max_seq_len)
+
+
 def attention_workspace_bytes(seq_count: int, q_heads: int, kv_heads: int, dim: int, max_seq_len: int) -> int:
     return lib().kvx_paged_attention_workspace_bytes(seq_count, q_heads, kv_heads, dim, max_seq_len)
 

@@ -10,7 +10,7 @@ from . import abi
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libkvx_b200.so")
 _lib = None
 
-# Every symbol include/kvx_abi.h, include/kvx_paged_kv.h and include/kvx_host.h declare.
+# Every symbol include/kvx_abi.h, the headers under include/ declare.
 EXPORTS = [
     "kvx_get_version", "kvx_validate_cache_desc", "kvx_write_kv", "kvx_gather_kv",
     "kvx_launch_write_kv", "kvx_launch_write_kv_prefill", "kvx_launch_gather_kv",
@@ -25,6 +25,9 @@ EXPORTS = [
     "kvx_host_pipe_sync", "kvx_host_pipe_traffic",
     "kvx_paged_attention_workspace_bytes", "kvx_launch_paged_attention_decode",
     "kvx_paged_attention_chunk_workspace_bytes", "kvx_launch_paged_attention_chunk", "kvx_attention_device_error",
+    "kvx_launch_rotary", "kvx_launch_rotary_write_kv",
+    "kvx_copy_pages_workspace_bytes", "kvx_launch_copy_pages", "kvx_launch_free_sequences", "kvx_fork_workspace_bytes",
+    "kvx_launch_fork_sequences", "kvx_launch_compact_pages",
 ]
 
 
@@ -74,6 +77,23 @@ def lib() -> C.CDLL:
                                                    P(abi.ScaleDesc), C.c_void_p, C.c_size_t, C.c_void_p]
     L.kvx_launch_paged_attention_chunk.restype = st
     L.kvx_attention_device_error.argtypes, L.kvx_attention_device_error.restype = [C.c_int], C.c_int
+    L.kvx_launch_rotary.argtypes, L.kvx_launch_rotary.restype = [P(abi.RotaryDesc), C.c_void_p], st
+    L.kvx_launch_rotary_write_kv.argtypes = [P(abi.CacheDesc), P(abi.WriteDesc), P(abi.RotaryDesc), C.c_void_p]
+    L.kvx_launch_rotary_write_kv.restype = st
+    L.kvx_copy_pages_workspace_bytes.argtypes, L.kvx_copy_pages_workspace_bytes.restype = [C.c_uint32], C.c_size_t
+    L.kvx_launch_copy_pages.argtypes = [P(abi.CacheDesc), C.c_uint32, C.c_void_p, C.c_void_p, C.c_int, C.c_uint32,
+                                        C.c_void_p, C.c_size_t, C.c_void_p]
+    L.kvx_launch_copy_pages.restype = st
+    L.kvx_launch_free_sequences.argtypes = [P(abi.BlockTable), P(abi.SeqLens), C.c_void_p, C.c_uint32, C.c_void_p,
+                                            C.c_uint32, C.c_void_p]
+    L.kvx_launch_free_sequences.restype = st
+    L.kvx_fork_workspace_bytes.argtypes, L.kvx_fork_workspace_bytes.restype = [C.c_uint32], C.c_size_t
+    L.kvx_launch_fork_sequences.argtypes = [P(abi.BlockTable), P(abi.SeqLens), C.c_void_p, C.c_uint32, C.c_uint32,
+                                            C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                            C.c_size_t, C.c_void_p]
+    L.kvx_launch_fork_sequences.restype = st
+    L.kvx_launch_compact_pages.argtypes = [P(abi.BlockTable), C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]
+    L.kvx_launch_compact_pages.restype = st
     L.kvx_kv_scales_workspace_bytes.argtypes, L.kvx_kv_scales_workspace_bytes.restype = [C.c_uint32], C.c_size_t
     L.kvx_launch_kv_scales.argtypes = [P(abi.KvIoDesc), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_size_t, C.c_void_p]

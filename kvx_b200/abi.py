@@ -115,10 +115,21 @@ class ChunkAttentionDesc(C.Structure):
                 ("seq_lens", SeqLens), ("query_indptr", C.c_void_p)]
 
 
+# KVX_ROTARY_* flags (include/kvx_rotary.h)
+ROTARY_INTERLEAVED, ROTARY_INVERSE = 1, 2
+
+
+class RotaryDesc(C.Structure):
+    """``kvx_rotary_desc_t`` (include/kvx_rotary.h)."""
+    _fields_ = [("size", C.c_uint32), ("rotary_dim", C.c_uint32), ("flags", C.c_uint32), ("position_dtype", C.c_int),
+                ("positions", C.c_void_p), ("inv_freq", C.c_void_p), ("factor", C.c_double), ("query", TensorDesc),
+                ("query_out", TensorDesc), ("key", TensorDesc), ("key_out", TensorDesc)]
+
+
 # x86-64 sizes frozen by the C header's static assertions.
 ABI_SIZES = {Version: 16, TensorDesc: 112, PoolDesc: 32, CacheDesc: 280, BlockTable: 64,
              SlotMapping: 32, SeqLens: 24, KvIoDesc: 248, ScaleDesc: 104, WriteDesc: 512,
-             GatherDesc: 352, AttentionDesc: 328, ChunkAttentionDesc: 344}
+             GatherDesc: 352, AttentionDesc: 328, ChunkAttentionDesc: 344, RotaryDesc: 488}
 for _cls, _bytes in ABI_SIZES.items():
     assert C.sizeof(_cls) == _bytes, (_cls.__name__, C.sizeof(_cls), _bytes)
 
@@ -300,3 +311,21 @@ def chunk_attention_desc(seq_count: int, rows: int, q_heads: int, dim: int, io_d
     a.seq_lens.dtype, a.seq_lens.seq_count, a.seq_lens.lengths = index_dtype, seq_count, lens_addr
     a.query_indptr_dtype, a.query_indptr = indptr_dtype, indptr_addr
     return a
+
+
+def block_table_desc(seq_count: int, max_blocks_per_seq: int, index_dtype: int, table_addr: int) -> BlockTable:
+    """A PACKED ``kvx_block_table_t``."""
+    b = BlockTable()
+    b.size = C.sizeof(BlockTable)
+    b.format, b.index_dtype, b.seq_count, b.beam_width = TABLE_PACKED, index_dtype, seq_count, 1
+    b.max_blocks_per_seq, b.indices = max_blocks_per_seq, table_addr
+    b.indices_count = (seq_count * max_blocks_per_seq) & 0xFFFFFFFF
+    return b
+
+
+def seq_lens_desc(seq_count: int, index_dtype: int, lens_addr: int) -> SeqLens:
+    """A ``kvx_seq_lens_t``."""
+    s = SeqLens()
+    s.size = C.sizeof(SeqLens)
+    s.dtype, s.seq_count, s.lengths = index_dtype, seq_count, lens_addr
+    return s

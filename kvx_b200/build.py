@@ -3,7 +3,8 @@
 The library holds the CUDA-free validators (``csrc/kvx_abi.c``), the launch layer and
 kernels (``csrc/kvx_paged_kv.cu``), the host-buffer pipeline (``csrc/kvx_host.cu``) and the decode
 attention over the paged cache (``csrc/kvx_attention.cu``), the attention of several new tokens
-(``csrc/kvx_chunk_attention.cu``),
+(``csrc/kvx_chunk_attention.cu``), rotary positions (``csrc/kvx_rotary.cu``) and page upkeep
+(``csrc/kvx_pages_ops.cu``),
 compiled for sm_100a only.  Run ``python -m kvx_b200.build`` or call :func:`build`.
 """
 from __future__ import annotations
@@ -22,7 +23,8 @@ BUILD_DIR = os.path.join(ROOT, "build")
 
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC", "-I" + INCLUDE]
-CU_SOURCES = ["kvx_paged_kv.cu", "kvx_host.cu", "kvx_attention.cu", "kvx_chunk_attention.cu"]
+CU_SOURCES = ["kvx_paged_kv.cu", "kvx_host.cu", "kvx_attention.cu", "kvx_chunk_attention.cu", "kvx_rotary.cu",
+              "kvx_pages_ops.cu"]
 
 
 def _nvcc() -> str:

@@ -15,6 +15,7 @@ packed caches and the prefill entry point, the descriptors are filled here throu
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 import re
 from typing import Optional
@@ -71,9 +72,18 @@ def _scale_arg(scale: Optional[torch.Tensor], device: torch.device) -> torch.Ten
     return t
 
 
+def _no_scratch(device: torch.device) -> torch.Tensor:
+    """An empty float32 tensor, standing for "no workspace given"."""
+    return _scale_arg(None, device)
+
+
 def _call_native(op, *args) -> None:
+    _returning_native(op, *args)
+
+
+def _returning_native(op, *args):
     try:
-        op(*args)
+        return op(*args)
     except RuntimeError as exc:
         m = _STATUS_RE.search(str(exc))
         if m is None:
@@ -360,7 +370,15 @@ def paged_attention_chunk(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     rows, q_heads, dim = query.shape
     if out is None:
         out = torch.empty((rows, q_heads, dim), dtype=query.dtype, device=query.device)
-    elif out.shape != query.shape or out.dtype != query.dtype:
+    native = native_ops() if key_cache.dim() == 4 and query.is_cuda else None
+    if native is not None:
+        dev = query.device
+        _call_native(native.paged_attention_chunk, out, query, key_cache, value_cache, block_table, seq_lens, query_indptr,
+                     float(scale), bool(causal), 0 if max_seq_len is None else int(max_seq_len), int(num_kv_heads or 0),
+                     _no_scratch(dev) if workspace is None else workspace, kv_cache_dtype, _scale_arg(k_scale, dev),
+                     _scale_arg(v_scale, dev))
+        return out
+    if out.shape != query.shape or out.dtype != query.dtype:
         raise ValueError("out must have the shape and dtype of query")
     for name, t in (("key_cache", key_cache), ("value_cache", value_cache), ("block_table", block_table),
                     ("seq_lens", seq_lens), ("query_indptr", query_indptr), ("out", out)):
@@ -398,6 +416,273 @@ def chunk_attention_workspace_bytes(seq_count: int, rows: int, q_heads: int, kv_
 
 def attention_workspace_bytes(seq_count: int, q_heads: int, kv_heads: int, dim: int, max_seq_len: int) -> int:
     return lib().kvx_paged_attention_workspace_bytes(seq_count, q_heads, kv_heads, dim, max_seq_len)
+
+
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none", scale: float = 1.0,
+                    original_length: int = 8192, low: float = 1.0, high: float = 4.0,
+                    device: Optional[torch.device] = None) -> tuple[torch.Tensor, float]:
+    """``(inv_freq, factor)`` for :func:`rotary_embedding`: float64 radians per position of the
+    ``rotary_dim / 2`` pairs, and the factor on the turned values.
+
+    ``scaling`` stretches a model trained on ``original_length`` positions by ``scale``:
+    ``"none"``; ``"linear"``, every frequency divided by ``scale``; ``"ntk"``, a larger base, so that
+    the slowest pair is divided by ``scale`` and the fastest kept; ``"bands"``, pairs that turn more
+    than ``high`` times over the original length kept, fewer than ``low`` times divided, linear in
+    the turns in between; ``"ramp"``, the same decision linear in the pair's index between the pairs
+    that turn ``high`` and ``low`` times, with the factor ``0.1 ln(scale) + 1``."""
+    if rotary_dim <= 0 or rotary_dim % 2 != 0:
+        raise ValueError("rotary_dim must be positive and even")
+    if not scale > 0 or not base > 1:
+        raise ValueError("scale must be positive and base above 1")
+    pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    factor = 1.0
+    if scaling == "ntk":
+        if rotary_dim <= 2:
+            raise ValueError("ntk scaling needs a rotary_dim above 2")
+        base = base * scale ** (rotary_dim / (rotary_dim - 2))
+    freq = base ** (-2.0 * pair / rotary_dim)
+    if scaling == "linear":
+        freq = freq / scale
+    elif scaling in ("bands", "ramp"):
+        if not high > low > 0:
+            raise ValueError("high and low must be turns with high > low > 0")
+        if scaling == "bands":
+            keep = (original_length * freq / (2 * math.pi) - low) / (high - low)
+        else:
+            at = [rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (high, low)]
+            first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim - 1)
+            keep = 1.0 - (pair - first) / max(last - first, 1e-3)
+            factor = 0.1 * math.log(scale) + 1.0 if scale > 1 else 1.0
+        keep = keep.clamp(0.0, 1.0)
+        freq = freq * keep + freq / scale * (1.0 - keep)
+    elif scaling not in ("none", "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return freq.to(device if device is not None else "cpu"), factor
+
+
+def _rotary_desc(query: Optional[torch.Tensor], query_out: Optional[torch.Tensor], tokens: int, device: torch.device,
+                 positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool, factor: float,
+                 inverse: bool) -> abi.RotaryDesc:
+    if positions.dtype not in _INDEX_CODES or positions.dim() != 1 or positions.numel() != tokens or not positions.is_contiguous():
+        raise ValueError("positions must hold one int32 or int64 per token")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float64 vector")
+    if positions.device != device or inv_freq.device != device:
+        raise ValueError("positions and inv_freq must be on the query's device")
+    r = abi.RotaryDesc()
+    r.size = C.sizeof(abi.RotaryDesc)
+    r.rotary_dim = 2 * inv_freq.numel()
+    r.flags = (abi.ROTARY_INTERLEAVED if interleaved else 0) | (abi.ROTARY_INVERSE if inverse else 0)
+    r.position_dtype, r.positions = _INDEX_CODES[positions.dtype], positions.data_ptr()
+    r.inv_freq, r.factor = inv_freq.data_ptr(), float(factor)
+    if query is not None:
+        code = _FLOAT_CODES[query.dtype]
+        r.query = abi.tensor_desc(query.data_ptr(), code, query.shape, query.stride(), abi.LAYOUT_INVALID)
+        r.query_out = abi.tensor_desc(query_out.data_ptr(), code, query_out.shape, query_out.stride(), abi.LAYOUT_INVALID)
+    return r
+
+
+def rotary_embedding(query: torch.Tensor, key: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
+                     interleaved: bool = False, factor: float = 1.0, inverse: bool = False,
+                     query_out: Optional[torch.Tensor] = None,
+                     key_out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotary positions (``include/kvx_rotary.h``): turns the first ``2 * len(inv_freq)`` dims of every
+    head of ``query`` (and ``key``, unless None) ``[tokens, heads, dim]`` by ``positions * inv_freq`` and
+    returns ``(query_out, key_out)``, new tensors unless given; ``query_out=query`` turns in place.
+    Token rows may be slices of wider rows.  ``inverse`` turns back: called on the gradients of the
+    outputs it gives those of the inputs.  ``inv_freq`` and ``factor`` as from
+    :func:`rotary_inv_freq`."""
+    if query.dim() != 3 or query.dtype not in _FLOAT_CODES or not query.is_cuda:
+        raise ValueError("query must be a [tokens, heads, dim] float CUDA tensor")
+    if key is not None and (key.dim() != 3 or key.dtype != query.dtype or key.device != query.device
+                            or key.shape[0] != query.shape[0] or key.shape[2] != query.shape[2]):
+        raise ValueError("key must match query in device, dtype, tokens and dim")
+    if query_out is None:
+        query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if key is not None and key_out is None:
+        key_out = torch.empty(key.shape, dtype=key.dtype, device=key.device)
+    native = native_ops()
+    if native is not None:
+        none = _no_scratch(query.device)
+        _call_native(native.rotary_embedding, query, none if key is None else key, positions, inv_freq, bool(interleaved),
+                     float(factor), bool(inverse), query_out, none if key is None else key_out)
+        return query_out, (None if key is None else key_out)
+    for t, o in ((query, query_out), (key, key_out)):
+        if t is not None and (o.shape != t.shape or o.dtype != t.dtype or o.device != t.device):
+            raise ValueError("an output must match its input")
+    r = _rotary_desc(query, query_out, query.shape[0], query.device, positions, inv_freq, interleaved, factor, inverse)
+    if key is not None:
+        code = _FLOAT_CODES[key.dtype]
+        r.key = abi.tensor_desc(key.data_ptr(), code, key.shape, key.stride(), abi.LAYOUT_INVALID)
+        r.key_out = abi.tensor_desc(key_out.data_ptr(), code, key_out.shape, key_out.stride(), abi.LAYOUT_INVALID)
+    with torch.cuda.device(query.device):
+        status = lib().kvx_launch_rotary(C.byref(r), _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx rotary", status)
+    return query_out, (None if key is None else key_out)
+
+
+def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
+                     inv_freq: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     slot_mapping: torch.Tensor, interleaved: bool = False, factor: float = 1.0,
+                     query_out: Optional[torch.Tensor] = None, kv_cache_dtype: str = "auto",
+                     k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`rotary_embedding` of ``query`` and ``key`` and :func:`reshape_and_cache_flash_kvx` of the
+    turned keys and of ``value`` in one pass: the pages hold the same bits, ``key`` stays as it is.
+    Returns ``query_out`` (new unless given; ``query`` itself turns in place).  Tokens with a negative
+    slot are turned but not cached."""
+    if query_out is None:
+        query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    native = native_ops() if key_cache.dim() == 4 else None
+    if native is not None:
+        dev = query.device
+        _call_native(native.rotary_and_cache, query, key, value, positions, inv_freq, key_cache, value_cache, slot_mapping,
+                     bool(interleaved), float(factor), query_out, kv_cache_dtype, _scale_arg(k_scale, dev),
+                     _scale_arg(v_scale, dev))
+        return query_out
+    if key.dim() != 3 or key.dtype not in _FLOAT_CODES or value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError("key/value must be matching [tokens, heads, dim] float tensors")
+    if query.dim() != 3 or query.dtype != key.dtype or query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2]:
+        raise ValueError("query must match key in dtype, tokens and dim")
+    if query_out.shape != query.shape or query_out.dtype != query.dtype:
+        raise ValueError("query_out must match query")
+    if slot_mapping.dtype not in _INDEX_CODES or slot_mapping.dim() != 1 or slot_mapping.numel() != key.shape[0] \
+            or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must hold one int32 or int64 slot per token")
+    for name, t in (("key", key), ("value", value), ("key_cache", key_cache), ("value_cache", value_cache),
+                    ("slot_mapping", slot_mapping), ("query_out", query_out)):
+        if not t.is_cuda or t.device != query.device:
+            raise ValueError(f"{name} must be on the query's CUDA device")
+    tokens, heads, dim = key.shape
+    cache = cache_desc_from_tensors(key_cache, value_cache, kv_cache_dtype, heads)
+    w = abi.write_desc(tokens, heads, dim, _FLOAT_CODES[key.dtype], key.data_ptr(), value.data_ptr(),
+                       _INDEX_CODES[slot_mapping.dtype], slot_mapping.data_ptr(), k_scale=_scale_desc(k_scale, heads),
+                       v_scale=_scale_desc(v_scale, heads))
+    for t, src in ((w.io.key, key), (w.io.value, value)):
+        for i, s in enumerate(src.stride()):
+            t.stride[i] = s
+    some = query.numel() > 0
+    r = _rotary_desc(query if some else None, query_out if some else None, tokens, query.device, positions, inv_freq,
+                     interleaved, factor, False)
+    with torch.cuda.device(query.device):
+        status = lib().kvx_launch_rotary_write_kv(C.byref(cache), C.byref(w), C.byref(r), _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx rotary write", status)
+    return query_out
+
+
+def _any_cache_desc(key_cache: torch.Tensor, value_cache: torch.Tensor) -> abi.CacheDesc:
+    """Page tensors by their strides alone: whole pages are moved, whatever their axes mean."""
+    if key_cache.shape != value_cache.shape or key_cache.dtype != value_cache.dtype:
+        raise ValueError("key/value cache mismatch")
+    kind = "fp8" if key_cache.dtype in _FP8_TORCH else "auto"
+    return cache_desc_from_tensors(key_cache, value_cache, kind, layout=abi.LAYOUT_NHD)
+
+
+def copy_pages(key_caches, value_caches, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copies page ``src[i]`` to page ``dst[i]`` in every key and value cache (lists, one entry per
+    layer), any dtype and layout, one launch for many layers (``include/kvx_pages_ops.h``).  Pairs
+    read the pages as they were before the call; pairs with a number outside the pool (``-1``
+    marks an unused entry), with a destination that a later pair names again, or with a source that
+    is a destination take no part."""
+    key_caches, value_caches = list(key_caches), list(value_caches)
+    if len(key_caches) != len(value_caches) or not key_caches:
+        raise ValueError("one value cache per key cache")
+    if src.dtype not in _INDEX_CODES or src.dim() != 1 or dst.shape != src.shape or dst.dtype != src.dtype or not src.is_cuda:
+        raise ValueError("src and dst must be matching int32 or int64 CUDA vectors")
+    native = native_ops()
+    if native is not None:
+        _call_native(native.copy_pages, key_caches, value_caches, src, dst)
+        return
+    if not src.is_contiguous() or not dst.is_contiguous():
+        raise ValueError("src and dst must be contiguous")
+    for t in [dst] + key_caches + value_caches:
+        if t.device != src.device:
+            raise ValueError("caches must be on the device of the page numbers")
+    caches = (abi.CacheDesc * len(key_caches))(*[_any_cache_desc(k, v) for k, v in zip(key_caches, value_caches)])
+    need = lib().kvx_copy_pages_workspace_bytes(src.numel())
+    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=src.device)
+    with torch.cuda.device(src.device):
+        status = lib().kvx_launch_copy_pages(caches, len(key_caches), src.data_ptr(), dst.data_ptr(), _INDEX_CODES[src.dtype],
+                                             src.numel(), scratch.data_ptr(), need, _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx page copy", status)
+
+
+def _table_args(block_table: torch.Tensor, seq_lens: Optional[torch.Tensor], page_refs: torch.Tensor, rows=()):
+    if block_table.dim() != 2 or not block_table.is_contiguous() or block_table.dtype not in _INDEX_CODES \
+            or not block_table.is_cuda:
+        raise ValueError("block_table must be a contiguous [seq_count, max_blocks_per_seq] int32 or int64 CUDA tensor")
+    dev, code = block_table.device, _INDEX_CODES[block_table.dtype]
+    if page_refs.dtype != torch.int32 or page_refs.dim() != 1 or not page_refs.is_contiguous() or page_refs.device != dev:
+        raise ValueError("page_refs must be a contiguous int32 vector on the table's device")
+    if seq_lens is not None and (seq_lens.dtype != block_table.dtype or seq_lens.shape != (block_table.shape[0],)
+                                 or not seq_lens.is_contiguous() or seq_lens.device != dev):
+        raise ValueError("seq_lens must have the table's dtype and one entry per row")
+    for r in rows:
+        if r.dtype != block_table.dtype or r.dim() != 1 or not r.is_contiguous() or r.device != dev:
+            raise ValueError("row numbers must be contiguous vectors of the table's dtype on its device")
+    t = abi.block_table_desc(block_table.shape[0], block_table.shape[1], code, block_table.data_ptr())
+    s = None if seq_lens is None else abi.seq_lens_desc(seq_lens.shape[0], code, seq_lens.data_ptr())
+    return t, s
+
+
+def free_sequences(block_table: torch.Tensor, seq_lens: torch.Tensor, page_refs: torch.Tensor, rows: torch.Tensor) -> None:
+    """Frees the table rows ``rows``: their pages give a reference back (``page_refs``, int32 per page,
+    0 = free), entries become -1 and lengths 0 (``include/kvx_pages_ops.h``)."""
+    native = native_ops() if block_table.is_cuda else None
+    if native is not None:
+        _call_native(native.free_sequences, block_table, seq_lens, page_refs, rows)
+        return
+    t, s = _table_args(block_table, seq_lens, page_refs, (rows,))
+    with torch.cuda.device(block_table.device):
+        status = lib().kvx_launch_free_sequences(C.byref(t), C.byref(s), page_refs.data_ptr(), page_refs.numel(),
+                                                 rows.data_ptr(), rows.numel(), _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx sequence free", status)
+
+
+def fork_sequences(block_table: torch.Tensor, seq_lens: torch.Tensor, page_refs: torch.Tensor, parents: torch.Tensor,
+                   children: torch.Tensor, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Forks row ``parents[i]`` into row ``children[i]``: full pages are shared, a partly filled last
+    page is duplicated into a free page (``include/kvx_pages_ops.h``).  Returns ``(src, dst)`` for
+    :func:`copy_pages`: -1 where nothing is to be copied, -2 where the pair was not forked (a row
+    outside the table or named twice, or no free page left; the child is then unchanged)."""
+    native = native_ops() if block_table.is_cuda else None
+    if native is not None:
+        return _returning_native(native.fork_sequences, block_table, seq_lens, page_refs, parents, children, int(block_size))
+    t, s = _table_args(block_table, seq_lens, page_refs, (parents, children))
+    if parents.numel() != children.numel():
+        raise ValueError("one child per parent")
+    n = parents.numel()
+    src, dst = torch.empty_like(parents), torch.empty_like(parents)
+    need = lib().kvx_fork_workspace_bytes(n)
+    scratch = torch.empty(max(need, 16), dtype=torch.uint8, device=block_table.device)
+    with torch.cuda.device(block_table.device):
+        status = lib().kvx_launch_fork_sequences(C.byref(t), C.byref(s), page_refs.data_ptr(), page_refs.numel(), int(block_size),
+                                                 parents.data_ptr(), children.data_ptr(), n, src.data_ptr(), dst.data_ptr(),
+                                                 scratch.data_ptr(), need, _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx sequence fork", status)
+    return src, dst
+
+
+def compact_pages(block_table: torch.Tensor, page_refs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Plans the move of all live pages to the front of the pool and renames them in ``block_table``
+    and ``page_refs`` (``include/kvx_pages_ops.h``).  Returns ``(src, dst)``, ``num_blocks // 2`` entries
+    with -1 behind the last move, for :func:`copy_pages`, to be run before the pages are read."""
+    native = native_ops() if block_table.is_cuda else None
+    if native is not None:
+        return _returning_native(native.compact_pages, block_table, page_refs)
+    t, _ = _table_args(block_table, None, page_refs)
+    n = max(1, page_refs.numel() // 2)
+    src, dst = (torch.empty(n, dtype=block_table.dtype, device=block_table.device) for _ in range(2))
+    with torch.cuda.device(block_table.device):
+        status = lib().kvx_launch_compact_pages(C.byref(t), page_refs.data_ptr(), page_refs.numel(), src.data_ptr(),
+                                                dst.data_ptr(), _stream())
+    if status != abi.STATUS_OK:
+        raise KvxError("kvx page compaction", status)
+    return src, dst
 
 
 def scales_workspace(heads: int, device: torch.device) -> torch.Tensor:

@@ -56,8 +56,16 @@ struct ChunkParams {
   int32_t grid, slot_rows, min_share;
   int32_t tile_rows, kv_tile;  // rows and tokens of one step of this kernel
   int32_t pair;                // 1: a tile of at most half the rows walks two K/V tiles per step
+  int32_t bs_shift;            // log2(block_size) or -1
   int32_t box;                 // tokens one TMA box loads
-  int32_t q_vec;               // 1: query rows can be read in 16-byte pieces
+  int32_t tile_cost;           // what a tile costs beyond its steps, in steps
+  // how K and V tiles lie in shared memory: bytes between groups of 8 tokens and between panels of 64 dims
+  int32_t group_stride, panel_stride;
+  int32_t whole_boxes;         // 1: a box carries all panels of its tokens, [8 tokens][panel]; 0: one panel
+  int32_t head_panels, head_groups;  // whole boxes: what a head adds to the panel and the group coordinate
+  int32_t head_inner;          // else: heads are closer together than tokens
+  int32_t q_tma;               // 1: query tiles are loaded by TMA
+  int32_t q_vec;               // 1: query rows can be read, out rows written in 16-byte pieces
   int32_t kv_vec;              // 1: page rows can be read in pieces of 8 elements
 };
 
@@ -111,7 +119,8 @@ __device__ __forceinline__ int32_t tiles_of(const ChunkParams &p, const Seq &q) 
 __device__ __forceinline__ bool is_narrow(const ChunkParams &p, const Seq &q) {
   return p.pair != 0 && q.rows * 2 <= p.tile_rows;
 }
-// K/V tiles and steps of row tile `t`.  A tile without any is still one step: its rows are written.
+// K/V tiles and steps of row tile `t`.  A tile without any is still one step: its rows are written;
+// loading its queries and writing its result count as `tile_cost` steps ahead of the first.
 __device__ __forceinline__ int32_t kv_tiles_of(const ChunkParams &p, const Seq &q, int32_t t) {
   const int32_t last = min(q.rows, (t + 1) * p.tile_rows) - 1;
   return (row_limit(p, q, last) + p.kv_tile - 1) / p.kv_tile;
@@ -119,7 +128,7 @@ __device__ __forceinline__ int32_t kv_tiles_of(const ChunkParams &p, const Seq &
 __device__ __forceinline__ int32_t steps_of(const ChunkParams &p, const Seq &q, int32_t t) {
   int32_t n = kv_tiles_of(p, q, t);
   if (is_narrow(p, q)) n = (n + 1) / 2;
-  return max(1, n);
+  return max(1, n) + p.tile_cost;
 }
 
 constexpr int kPlanThreads = 1024;
@@ -194,6 +203,12 @@ __device__ __forceinline__ int shares(const ChunkParams &p, int64_t total) {
 __device__ __forceinline__ int64_t share_begin(int64_t total, int n, int c) {
   return total * c / n;  // total < 2^48, n < 2^15
 }
+// A cut at `at` inside the tile [begin, end) goes to the tile's edge where it would leave next to
+// nothing on one side.
+__device__ __forceinline__ int64_t snap(const ChunkParams &p, int64_t at, int64_t begin, int64_t end) {
+  if (at - begin <= p.tile_cost + 1) return begin;
+  return end - at <= 1 ? end : at;
+}
 
 // All lanes of a warp call it together and get the same answer.  `at` < prefix[seq_count].
 __device__ Place find_place(const ChunkParams &p, int64_t at) {
@@ -238,6 +253,26 @@ __device__ Place find_place(const ChunkParams &p, int64_t at) {
   }
 }
 
+// Share `share` of the schedule: from `w` on, `left` steps.
+__device__ __forceinline__ int64_t find_share(const ChunkParams &p, int share, Place *w) {
+  const int64_t total = p.prefix[p.seq_count];
+  const int n = shares(p, total);
+  if (share >= n) return 0;
+  int64_t at[2];
+  Place e[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    at[i] = share_begin(total, n, share + i);
+    if (at[i] >= total) continue;
+    e[i] = find_place(p, at[i]);
+    const int64_t begin = at[i] - e[i].off, to = snap(p, at[i], begin, begin + e[i].steps);
+    e[i].off = static_cast<int32_t>(to - begin);
+    at[i] = to;
+  }
+  *w = e[0];
+  return at[1] - at[0];
+}
+
 // The next tile after w's, in the order of the schedule; w.seq = seq_count when there is none.
 __device__ __forceinline__ void next_tile(const ChunkParams &p, Place &w) {
   w.off = 0;
@@ -273,8 +308,8 @@ __device__ __forceinline__ Piece piece_of(const ChunkParams &p, const Place &w, 
   x.narrow = is_narrow(p, w.q) ? 1 : 0;
   const int32_t n = kv_tiles_of(p, w.q, w.tile);
   const int32_t mul = x.narrow ? 2 : 1;
-  x.kv0 = min(n, w.off * mul);
-  x.kv1 = min(n, end * mul);
+  x.kv0 = min(n, max(0, w.off - p.tile_cost) * mul);
+  x.kv1 = min(n, max(0, end - p.tile_cost) * mul);
   // a share holds at most one piece that continues a tile begun earlier and one that begins a
   // tile ended later
   x.slot = (w.off == 0 && end == w.steps) ? -1 : (w.off > 0 ? 2 * share : 2 * share + 1);
@@ -316,7 +351,7 @@ __device__ __forceinline__ int64_t head_offset(const PageView &v, int64_t o, int
 
 // Page of token `tok` of sequence `seq`, -1 when it takes no part.
 __device__ __forceinline__ int32_t page_of(const ChunkParams &p, int32_t seq, int32_t tok) {
-  const int32_t lb = tok / p.block_size;
+  const int32_t lb = p.bs_shift >= 0 ? tok >> p.bs_shift : tok / p.block_size;
   if (lb >= p.max_blocks) return -1;
   const int64_t b = read_index(p.table, static_cast<int64_t>(seq) * p.max_blocks + lb, p.table64);
   return b < 0 || b >= p.num_blocks ? -1 : static_cast<int32_t>(b);
@@ -330,9 +365,10 @@ __device__ __forceinline__ float score_mul(const ChunkParams &p, int head) {
   return p.ks.base != nullptr ? p.scale_log2 * p.ks.base[head * p.ks.stride] : p.scale_log2;
 }
 
-// The kernels keep scores of a query whose sign makes the multiplier positive; a multiplier of zero
-// becomes a query of zeros (zero times the -inf of a masked score would be a NaN).
-__device__ __forceinline__ float score_abs(float mul) { return mul == 0.f ? 1.f : fabsf(mul); }
+// Running maxima are kept of scores times the sign of the multiplier, and weighted with its size.  A
+// multiplier of zero (zero times the -inf of a masked score would be a NaN) is taken as 2^-126, which
+// makes every score's exponent zero all the same.
+__device__ __forceinline__ float nonzero(float mul) { return mul == 0.f ? 1.17549435e-38f : mul; }
 
 // ------------------------------------------------------------------ merge of pieces ----
 
@@ -346,17 +382,23 @@ __global__ void __launch_bounds__(kMergeThreads) kvx_chunk_merge_kernel(const Ch
   const int n = shares(p, total);
   const int cut = blockIdx.x + 1;
   if (cut >= n) return;
-  const int64_t at = share_begin(total, n, cut);
-  const Place w = find_place(p, at);
-  if (w.off == 0) return;
-  const int64_t tile_at = at - w.off, tile_end = tile_at + w.steps;
-  if (share_begin(total, n, cut - 1) > tile_at) return;  // an earlier cut goes through this tile
+  const int64_t raw = share_begin(total, n, cut);
+  const Place w = find_place(p, raw);
+  const int64_t tile_at = raw - w.off, tile_end = tile_at + w.steps;
+  const int64_t at = snap(p, raw, tile_at, tile_end);
+  if (at == tile_at || at == tile_end) return;
+  const int64_t ahead = share_begin(total, n, cut - 1);
+  if (ahead > tile_at && snap(p, ahead, tile_at, tile_end) > tile_at) return;  // an earlier cut goes through this tile
   // shares cut .. last continue the tile, share cut - 1 began it
   int last = cut;
-  while (last + 1 < n && share_begin(total, n, last + 1) < tile_end) ++last;
+  while (last + 1 < n) {
+    const int64_t next = share_begin(total, n, last + 1);
+    if (next >= tile_end || snap(p, next, tile_at, tile_end) == tile_end) break;
+    ++last;
+  }
   const int32_t row0 = w.tile * p.tile_rows, rows = min(p.tile_rows, w.q.rows - row0);
   const int lane = threadIdx.x & 31;
-  const float mul = score_abs(score_mul(p, w.head));
+  const float mul = fabsf(nonzero(score_mul(p, w.head)));
   for (int r = blockIdx.y * (kMergeThreads / 32) + (threadIdx.x >> 5); r < rows; r += gridDim.y * (kMergeThreads / 32)) {
     float m = -INFINITY;
     for (int c = cut - 1 + lane; c <= last; c += 32) {
@@ -387,6 +429,11 @@ __global__ void __launch_bounds__(kMergeThreads) kvx_chunk_merge_kernel(const Ch
 
 // ------------------------------------------------------------------ mbarriers, TMA, tensor memory --
 
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t e;
+  asm volatile("{ .reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p; }" : "=r"(e));
+  return e;
+}
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -408,66 +455,83 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
-
-// Waits for the phase; after two seconds, or when another warp gave up, sets the CTA's flag and
-// answers false, upon which every role returns.  (Inlined: a call here would have to save the
-// scores a softmax thread holds in registers.)
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t from = now_ns();
-#pragma unroll 1
-  for (;;) {
-#pragma unroll 1
-    for (int i = 0; i < 64; ++i)
-      if (mbar_try(bar, parity)) return true;
-    if (*gave_up != 0) return false;
-    if (now_ns() - from > kWaitLimitNs) {
-      *gave_up = 1;
-      g_chunk_error = 1;
-      return false;
-    }
-  }
-}
-// The same for a whole warp: all lanes get one answer.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
-  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, gave_up)) != 0;
-}
-
-__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap *map, int x, int c1, int c2, int c3, uint32_t bar) {
+// Waits for the phase, at most two seconds (kTries suspensions of up to a microsecond); a wait that
+// gives up sets the device's word and answers false, upon which its role returns.  Few
+// instructions on purpose, see the note at the kernel.
+constexpr uint32_t kTries = 2000000;
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      "{ .reg .pred p;\n\t"
+      ".reg .u32 n;\n\t"
+      "mov.u32 n, %3;\n\t"
+      "AGAIN:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
+      "@p bra DONE;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 p, n, 0;\n\t"
+      "@p bra AGAIN;\n\t"
+      "DONE:\n\t"
+      "selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "n"(kTries), "r"(1000u)
+      : "memory");
+  if (ok == 0) g_chunk_error = 1;
+  return ok != 0;
+}
+// The same for a whole warp: all lanes get one answer, and the compiler knows that they do.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity)) != 0;
+}
+
+// Issued by the elected lane of a warp whose lanes agree on all operands.
+__device__ __forceinline__ void tma_load4(uint32_t elected, uint32_t dst, const CUtensorMap *map, int x, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred q;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6]; }" ::"r"(dst),
+      "l"(map), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load5(uint32_t elected, uint32_t dst, const CUtensorMap *map, int panel, int group, int page, uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%7, %7, %2, %3, %4}], [%5]; }" ::"r"(dst),
+      "l"(map), "r"(panel), "r"(group), "r"(page), "r"(bar), "r"(elected), "r"(0)
       : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// d[128 x N] (+)= a[128 x 16] b[N x 16]^T; a and b in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_commit(uint32_t elected, uint32_t bar) {
   asm volatile(
-      "{ .reg .pred p;\n\t"
+      "{ .reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar), "r"(elected)
+      : "memory");
+}
+// d[128 x N] (+)= a[128 x 16] b[N x 16]^T; a and b in shared memory.  Called by a whole warp, issued by
+// the elected lane: in code that the compiler can see to be uniform, descriptors live in uniform
+// registers, which is where the instruction wants them.
+__device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
       : "memory");
 }
 // the same with a in tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{ .reg .pred p;\n\t"
+      "{ .reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
       : "memory");
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -485,7 +549,19 @@ __device__ __forceinline__ void tc_ld32(float *x, uint32_t at) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(at));
 }
-__device__ __forceinline__ void tc_ld16(uint32_t *r, uint32_t at) {
+__device__ __forceinline__ void tc_st32(uint32_t at, const float *x) {
+  const uint32_t *r = reinterpret_cast<const uint32_t *>(x);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tc_ld16(float *x, uint32_t at) {
+  uint32_t *r = reinterpret_cast<uint32_t *>(x);
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -499,7 +575,11 @@ __device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t *r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-
+__device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // Shared-memory operand descriptor, 128-byte swizzle: rows of 128 bytes, 8 of them to an atom of
 // 1 024 bytes.  `stride` bytes between groups of 8 rows; `lead` bytes between blocks of 64
 // elements along the rows (used when the rows run along the reduction, i.e. for V).
@@ -538,9 +618,10 @@ struct Fp16 {
 //
 // Roles of a CTA (one per SM, 384 threads):
 //   warps 0-3, 4-7   softmax of stream 0 and of stream 1: a thread owns one of the 128 rows
-//   warp 8           one thread issues every tcgen05.mma
-//   warp 9           walks the schedule, publishes pieces, loads K and V tiles (TMA)
-//   warps 10, 11     help loading where pages cannot be read by TMA
+//   warp 8           issues every tcgen05.mma
+//   warp 9           walks the schedule, publishes pieces, loads Q and K tiles (TMA)
+//   warp 10          loads V tiles
+//   (warps 9 to 11   copy K and V tiles where pages cannot be read by TMA)
 // Two streams of 128 rows keep the tensor pipe and the exponentials busy in turn: while one
 // stream's scores are turned into weights the other stream's products run.  A tile with at most
 // 128 rows gives both streams the same rows and every K/V tile to one of them; the two halves are
@@ -553,6 +634,7 @@ struct Fp16 {
 // the previous product read.
 
 constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8;
 constexpr int kTile = 128;          // rows of a stream, tokens of a K/V tile
 constexpr int kPanelBytes = 16384;  // 128 rows x 128 bytes
 constexpr int kItems = 2;           // pieces published ahead
@@ -563,23 +645,23 @@ struct Shape {
   static constexpr int kScoreBufs = kDp > 128 ? 2 : 1;     // per stream
   static constexpr int kPanels = kDp / 64;                 // 64 dims (128 bytes) each
   static constexpr int kUnitPanels = kPanels > 2 ? 2 : kPanels;
-  static constexpr int kUnits = kPanels / kUnitPanels;     // ring entries per K (or V) tile
+  static constexpr int kUnits = kPanels / kUnitPanels;     // ring entries per tile
   static constexpr int kUnitBytes = kUnitPanels * kPanelBytes;
-  static constexpr int kStages = kDp == 64 ? 8 : 5;
+  static constexpr int kRing = kDp == 64 ? 4 : 2;          // entries of the K ring and of the V ring (powers of two)
   static constexpr int kQBytes = kPanels * kPanelBytes;    // per stream
   static constexpr int kRingAt = kStreams * kQBytes;
-  static constexpr int kMiscAt = kRingAt + kStages * kUnitBytes;
+  static constexpr int kMiscAt = kRingAt + 2 * kRing * kUnitBytes;
 };
 
 struct Misc {
   uint64_t item_full[kItems], item_empty[kItems];
   uint64_t kv_full[8], kv_empty[8];
-  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
-  uint64_t tail, drain, join_full, join_empty;
+  uint64_t q_full[2], q_empty[2], s_full[2], p_part[2], p_full[2], pv_done[2];
+  uint64_t join_full, join_empty;
+  uint64_t tail, drain;
   Piece items[kItems];
   float join_m[kTile], join_l[kTile];
   uint32_t tmem;
-  int gave_up;
 };
 
 template <int kDp>
@@ -603,149 +685,202 @@ __device__ __forceinline__ void stream_range(const ChunkParams &p, const Piece &
   *e = max(x.kv0, min(x.kv1, (limit + kTile - 1) / kTile));
 }
 
-// Loads the K and V tiles of a piece in the order in which Products::piece consumes them.
-template <int kStreams, typename Load>
-__device__ __forceinline__ bool walk_loads(const ChunkParams &p, const Piece &x, Load &&load) {
+// The K tiles (and the V tiles) of a piece in the order in which they are consumed: one after the
+// other, or for a narrow piece from the two streams in turn.
+struct TileOrder {
+  int32_t b0, b1, count, narrow;
+  __device__ __forceinline__ int32_t tile(int q) const { return narrow ? ((q & 1) ? b1 : b0) + (q >> 1) : b0 + q; }
+};
+template <int kStreams>
+__device__ __forceinline__ TileOrder tile_order(const ChunkParams &p, const Piece &x) {
   int b0, e0, b1 = 0, e1 = 0;
   stream_range<kStreams>(p, x, 0, &b0, &e0);
   if (kStreams == 2) stream_range<kStreams>(p, x, 1, &b1, &e1);
-  if (kStreams == 1) {
-    const int n = e0 - b0;
-    if (n > 0 && !load(false, b0)) return false;
-    for (int i = 0; i < n; ++i) {
-      if (i + 1 < n && !load(false, b0 + i + 1)) return false;
-      if (!load(true, b0 + i)) return false;
-    }
-    return true;
-  }
-  if (x.narrow) {
-    const int n0 = e0 - b0, n1 = e1 - b1;
-    if (n0 > 0 && !load(false, b0)) return false;
-    if (n1 > 0 && !load(false, b1)) return false;
-    for (int i = 0; i < n0; ++i) {
-      if (!load(true, b0 + i)) return false;
-      if (i + 1 < n0 && !load(false, b0 + i + 1)) return false;
-      if (i < n1 && !load(true, b1 + i)) return false;
-      if (i + 1 < n1 && !load(false, b1 + i + 1)) return false;
-    }
-    return true;
-  }
-  const int n = max(e0, e1) - x.kv0;
-  if (n > 0 && !load(false, x.kv0)) return false;
-  for (int i = 0; i < n; ++i) {
-    if (!load(true, x.kv0 + i)) return false;
-    if (i + 1 < n && !load(false, x.kv0 + i + 1)) return false;
+  const bool narrow = kStreams == 2 && x.narrow;
+  return TileOrder{narrow ? b0 : x.kv0, b1, narrow ? (e0 - b0) + (e1 - b1) : max(e0, e1) - x.kv0, narrow ? 1 : 0};
+}
+
+// Whether stream 1 hands its half of a narrow tile to stream 0 (it has K/V tiles of its own).
+__device__ __forceinline__ bool joins_streams(const Piece &x) { return x.narrow && x.kv1 - x.kv0 > 1; }
+
+__device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap *map, int x, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+// Query tiles of a piece by TMA, one lane: `group` is a power of two, so the 128 rows of a stream are
+// the group's heads of 128 / group whole tokens.  Rows behind the sequence are other sequences'
+// or zeros; nothing is written for them.
+template <int kDp>
+__device__ bool load_queries(const ChunkParams &p, const CUtensorMap *qmap, const Piece &x, uint32_t base, Misc *m, uint32_t *count) {
+  using S = Shape<kDp>;
+  for (int s = 0; s < S::kStreams; ++s) {
+    int b, e;
+    stream_range<S::kStreams>(p, x, s, &b, &e);
+    if (e == b) continue;
+    const uint32_t bar = smem_addr(&m->q_full[s]);
+    if (count[s] > 0 && !mbar_wait(smem_addr(&m->q_empty[s]), (count[s] - 1) & 1)) return false;
+    ++count[s];
+    mbar_expect_tx(bar, S::kQBytes);
+    const int32_t token = x.q.first + (x.row0 + (x.narrow ? 0 : s * kTile)) / p.group;
+    for (int k = 0; k < S::kPanels; ++k)
+      tma_load3(base + s * S::kQBytes + k * kPanelBytes, qmap, k * 64, x.head * p.group, token, bar);
   }
   return true;
 }
 
+// Place in the K ring (0) or the V ring (1): entries are used in turn.
+template <int kDp>
 struct Ring {
-  uint32_t stage = 0, phase = 0;
-  template <int kStages>
-  __device__ __forceinline__ void next() {
-    if (++stage == kStages) stage = 0, phase ^= 1;
-  }
+  using S = Shape<kDp>;
+  uint32_t at;     // the ring's first entry in shared memory
+  uint32_t first;  // its first barrier's number
+  uint32_t entry = 0;
+  __device__ __forceinline__ Ring(uint32_t base, int which) : at(base + S::kRingAt + which * S::kRing * S::kUnitBytes), first(which * S::kRing) {}
+  __device__ __forceinline__ uint32_t slot() const { return first + (entry & (S::kRing - 1)); }
+  __device__ __forceinline__ uint32_t addr() const { return at + (entry & (S::kRing - 1)) * S::kUnitBytes; }
+  __device__ __forceinline__ uint32_t phase() const { return entry / S::kRing & 1; }
 };
 
 // ---- loads ------------------------------------------------------------------------------
 
+// Two warps load by TMA: the first walks the schedule, publishes the pieces, loads the queries and the
+// K tiles, the second loads the V tiles.  What a single warp does per box and per tile is on the
+// kernel's critical path (one instruction every ten clocks or so), so a box carries all panels of
+// its tokens where the layout allows, its coordinates are looked up a tile ahead, one box per lane,
+// and the boxes are issued by one lane of converged code.
 template <int kDp>
-__device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, uint32_t base, Misc *m) {
+__device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, const CUtensorMap *qmap, uint32_t base,
+                              Misc *m, bool mine_v) {
   using S = Shape<kDp>;
   const int lane = threadIdx.x & 31;
-  volatile int *gave_up = &m->gave_up;
-  Ring ring;
-  uint32_t loads = 0;  // ring entries filled so far
+  const uint32_t elected = elect_lane();
+  Ring<kDp> ring(base, mine_v ? 1 : 0);
+  uint32_t queries[2] = {0, 0};
   uint32_t tail_phase = 0;
   const int boxes = kTile / p.box;
-  const int64_t total = p.prefix[p.seq_count];
-  const int n = shares(p, total), share = blockIdx.x;
+  const CUtensorMap *map = mine_v ? vmap : kmap;
+  const uint32_t box_bytes = p.box / 8 * p.group_stride;
+  // Page of this lane's box of a tile (beyond the sequence, or where there is no such page, a number
+  // behind the pool, which TMA answers with zeros), and its first token's place in the page.
+  auto look_up = [&](const Piece &x, int tile, int32_t *in_page) {
+    const int32_t tok = tile * kTile + lane * p.box;
+    *in_page = 0;
+    if (lane >= boxes || tok >= x.q.len) return p.num_blocks;
+    const int32_t page = page_of(p, x.seq, tok);
+    *in_page = p.bs_shift >= 0 ? tok & (p.block_size - 1) : tok % p.block_size;
+    return page >= 0 ? page : p.num_blocks;
+  };
+  auto load_piece = [&](const Piece &x) {
+    const TileOrder order = tile_order<S::kStreams>(p, x);
+    const int32_t c_panel = x.head * p.head_panels, c_group = x.head * p.head_groups;
+    int32_t in_page = 0, page = p.num_blocks;
+#pragma unroll 1
+    for (int q = -1; q < order.count; ++q) {
+      const int32_t now_page = page, now_in = in_page;
+      page = look_up(x, order.tile(min(q + 1, order.count - 1)), &in_page);
+      if (q < 0) continue;
+      const int tile = order.tile(q);
+      const int valid = x.q.len - tile * kTile;  // tokens of the tile that exist
+      const bool tail = __any_sync(0xFFFFFFFFu, mine_v && valid < kTile && valid % p.box != 0) != 0;
+#pragma unroll 1
+      for (int u = 0; u < S::kUnits; ++u, ++ring.entry) {
+        const uint32_t st = ring.slot();
+        if (ring.entry >= S::kRing && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase() ^ 1)) return false;
+        uint32_t dst = ring.addr();
+        const uint32_t bar = smem_addr(tail ? &m->tail : &m->kv_full[st]);
+        if (elected) mbar_expect_tx(bar, S::kUnitBytes);
+        __syncwarp();
+        if (p.whole_boxes) {
+#pragma unroll 2
+          for (int k = 0; k < boxes; ++k, dst += box_bytes)
+            tma_load5(elected, dst, map, c_panel + u * S::kUnitPanels, c_group + (__shfl_sync(0xFFFFFFFFu, now_in, k) >> 3),
+                      __shfl_sync(0xFFFFFFFFu, now_page, k), bar);
+        } else {
+          const bool head_inner = p.head_inner != 0;
+#pragma unroll 1
+          for (int k = 0; k < boxes; ++k, dst += box_bytes) {
+            const int32_t pg = __shfl_sync(0xFFFFFFFFu, now_page, k), in = __shfl_sync(0xFFFFFFFFu, now_in, k);
+#pragma unroll
+            for (int pp = 0; pp < S::kUnitPanels; ++pp)
+              tma_load4(elected, dst + pp * kPanelBytes, map, (u * S::kUnitPanels + pp) * 64, head_inner ? x.head : in,
+                        head_inner ? in : x.head, pg, bar);
+          }
+        }
+        if (tail) {
+          // Rows of the last page behind the sequence hold whatever the page holds; their weight
+          // is zero, but zero times a NaN is not: overwrite them.
+          if (!warp_wait(bar, tail_phase)) return false;
+          tail_phase ^= 1;
+          const int rows = min(kTile, (valid + p.box - 1) / p.box * p.box) - valid;
+#pragma unroll 1
+          for (int i = lane; i < rows * 8 * S::kUnitPanels; i += 32) {
+            const int row = valid + i / (8 * S::kUnitPanels), c = i % (8 * S::kUnitPanels);
+            const uint32_t to = ring.addr() + (row >> 3) * p.group_stride + (row & 7) * 128 + (c >> 3) * p.panel_stride + (c & 7) * 16;
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(to), "r"(0u) : "memory");
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (elected) mbar_arrive(smem_addr(&m->kv_full[st]));
+        }
+      }
+    }
+    return true;
+  };
   bool ok = true;
-  uint32_t item = 0;
-  if (share < n) {
-    int64_t at = share_begin(total, n, share);
-    const int64_t end = share_begin(total, n, share + 1);
-    Place w = find_place(p, at);
-    while (ok && at < end) {
-      const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + (end - at)));
-      const Piece x = piece_of(p, w, stop, share);
-      const uint32_t slot = item % kItems;
-      if (item >= kItems) ok = warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up);
+  Place w;
+  int64_t left = 0;
+  if (!mine_v) {
+    left = find_share(p, blockIdx.x, &w);
+    if (left > 0 && w.off >= w.steps) next_tile(p, w);
+  }
+#pragma unroll 1
+  for (uint32_t item = 0;; ++item) {
+    const uint32_t slot = item % kItems;
+    Piece x;
+    if (mine_v) {
+      ok = warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1);
       if (!ok) break;
-      if (lane == 0) {
+      x = m->items[slot];
+      __syncwarp();
+      if (elected) mbar_arrive(smem_addr(&m->item_empty[slot]));
+    } else {
+      // one piece more than there is, without rows: the end
+      if (item >= kItems) ok = warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1);
+      if (!ok) break;
+      x.rows = 0;
+      if (left > 0) {
+        const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
+        x = piece_of(p, w, stop, blockIdx.x);
+        left -= stop - w.off;
+        if (left > 0) next_tile(p, w);
+      }
+      if (elected) {
         m->items[slot] = x;
         mbar_arrive(smem_addr(&m->item_full[slot]));
       }
-      ++item;
-      ok = walk_loads<S::kStreams>(p, x, [&](bool is_v, int tile) {
-        // every lane < boxes owns one box: its page, or (beyond the sequence, no such page) a page
-        // number behind the pool, which TMA answers with zeros
-        int32_t page = p.num_blocks, in_page = 0;
-        if (lane < boxes) {
-          const int32_t tok = tile * kTile + lane * p.box;
-          if (tok < x.q.len) {
-            const int32_t b = page_of(p, x.seq, tok);
-            if (b >= 0) page = b, in_page = tok % p.block_size;
-          }
-        }
-        const int valid = x.q.len - tile * kTile;  // tokens of the tile that exist
-        const bool tail = is_v && valid < kTile && valid % p.box != 0;
-        const bool head_inner = p.k.head < p.k.tok;  // order of the map's middle dimensions
-        for (int u = 0; u < S::kUnits; ++u) {
-          const uint32_t st = ring.stage;
-          if (loads >= S::kStages && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase ^ 1, gave_up)) return false;
-          const uint32_t dst = base + S::kRingAt + st * S::kUnitBytes;
-          const uint32_t bar = smem_addr(tail ? &m->tail : &m->kv_full[st]);
-          if (lane == 0) mbar_expect_tx(bar, S::kUnitBytes);
-          __syncwarp();
-          if (lane < boxes) {
-            for (int pp = 0; pp < S::kUnitPanels; ++pp) {
-              const int x0 = (u * S::kUnitPanels + pp) * 64;
-              tma_load4(dst + pp * kPanelBytes + lane * p.box * 128, is_v ? vmap : kmap, x0, head_inner ? x.head : in_page,
-                        head_inner ? in_page : x.head, page, bar);
-            }
-          }
-          if (tail) {
-            // Rows of the last page behind the sequence hold whatever the page holds; their weight
-            // is zero, but zero times a NaN is not: overwrite them.
-            if (!warp_wait(bar, tail_phase, gave_up)) return false;
-            tail_phase ^= 1;
-            const int upto = min(kTile, (valid + p.box - 1) / p.box * p.box);
-            for (int i = lane; i < (upto - valid) * 8 * S::kUnitPanels; i += 32) {
-              const int pp = i / ((upto - valid) * 8), j = i - pp * (upto - valid) * 8;
-              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(dst + pp * kPanelBytes + valid * 128 + j * 16), "r"(0u)
-                           : "memory");
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_addr(&m->kv_full[st]));
-          }
-          ring.next<S::kStages>();
-          ++loads;
-        }
-        return true;
-      });
-      at += stop - w.off;
-      if (at < end) next_tile(p, w);
+      __syncwarp();
     }
-  }
-  if (ok) {
-    const uint32_t slot = item % kItems;
-    if (item >= kItems) ok = warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up);
-    if (ok && lane == 0) {
-      m->items[slot].rows = 0;  // no more pieces
-      mbar_arrive(smem_addr(&m->item_full[slot]));
+    if (__all_sync(0xFFFFFFFFu, x.rows == 0)) break;
+    if (!mine_v && p.q_tma) {
+      if (elected) ok = load_queries<kDp>(p, qmap, x, base, m, queries);
+      ok = __all_sync(0xFFFFFFFFu, ok) != 0;
+      if (!ok) break;
     }
+    ok = load_piece(x);
+    if (!ok) break;
   }
   // Nothing may be in flight towards this CTA's shared memory when it ends.  Normally: every
   // entry's release has arrived.  After giving up: the loads themselves, as far as they come.
-  const uint32_t held = min(loads, static_cast<uint32_t>(S::kStages));
-  for (uint32_t k = 0; k < held; ++k) {
-    const uint32_t entry = loads - held + k, st = entry % S::kStages, ph = (entry / S::kStages) & 1;
-    if (ok) ok = warp_wait(smem_addr(&m->kv_empty[st]), ph, gave_up);
+  const uint32_t held = min(ring.entry, static_cast<uint32_t>(S::kRing)), end = ring.entry;
+#pragma unroll 1
+  for (ring.entry = end - held; ring.entry != end; ++ring.entry) {
+    if (ok) ok = warp_wait(smem_addr(&m->kv_empty[ring.slot()]), ring.phase());
     if (!ok) {
       int ignore = 0;
-      for (int i = 0; i < 4096 && ignore == 0; ++i) ignore = mbar_try(smem_addr(&m->kv_full[st]), ph) ? 1 : 0;
+      for (int i = 0; i < 4096 && ignore == 0; ++i) ignore = mbar_try(smem_addr(&m->kv_full[ring.slot()]), ring.phase()) ? 1 : 0;
     }
   }
 }
@@ -753,40 +888,44 @@ __device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, con
 // Pages that TMA cannot read (e4m3, HND_PACKED, odd page sizes, odd strides): three warps copy rows
 // into the same swizzled tiles, converting on the way.  Warp 9 walks the schedule here, too.
 template <typename T, int kDp>
-__device__ void load_role_copy(const ChunkParams &p, uint32_t base, Misc *m) {
+__device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, uint32_t base, Misc *m) {
   using S = Shape<kDp>;
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - 9, tid = threadIdx.x - 9 * 32;
-  volatile int *gave_up = &m->gave_up;
-  Ring ring;
-  uint32_t loads = 0, item = 0;
-  const int64_t total = p.prefix[p.seq_count];
-  const int n = shares(p, total), share = blockIdx.x;
-  int64_t at = 0, end = 0;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - (kMmaWarp + 1), tid = threadIdx.x - (kMmaWarp + 1) * 32;
+  Ring<kDp> rings[2] = {Ring<kDp>(base, 0), Ring<kDp>(base, 1)};
+  uint32_t item = 0, queries[2] = {0, 0};
+  const int share = blockIdx.x;
   Place w;
-  if (share < n) {
-    at = share_begin(total, n, share);
-    end = share_begin(total, n, share + 1);
-    w = find_place(p, at);
-  }
+  int64_t left = find_share(p, share, &w);
+  if (left > 0 && w.off >= w.steps) next_tile(p, w);
   const int elem = elem_bytes(p.cache_code);
-  while (at < end) {
-    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + (end - at)));
+  while (left > 0) {
+    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
     const Piece x = piece_of(p, w, stop, share);
     if (warp == 0) {
       const uint32_t slot = item % kItems;
-      if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up)) return;
+      if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1)) return;
+      bool ok = true;
       if (lane == 0) {
         m->items[slot] = x;
         mbar_arrive(smem_addr(&m->item_full[slot]));
+        if (p.q_tma) ok = load_queries<kDp>(p, qmap, x, base, m, queries);
       }
+      if (!__all_sync(0xFFFFFFFFu, ok)) return;
     }
     ++item;
-    const bool ok = walk_loads<S::kStreams>(p, x, [&](bool is_v, int tile) {
+    const TileOrder order = tile_order<S::kStreams>(p, x);
+    // (a V tile is consumed after the K tile behind it has been asked for)
+#pragma unroll 1
+    for (int q = 0; q < 2 * order.count; ++q) {
+      const bool is_v = (q & 1) != 0;
+      const int tile = order.tile(q >> 1);
       const PageView &view = is_v ? p.v : p.k;
-      for (int u = 0; u < S::kUnits; ++u) {
-        const uint32_t st = ring.stage;
-        if (loads >= S::kStages && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase ^ 1, gave_up)) return false;
-        const uint32_t dst = base + S::kRingAt + st * S::kUnitBytes;
+      Ring<kDp> &ring = rings[is_v];
+#pragma unroll 1
+      for (int u = 0; u < S::kUnits; ++u, ++ring.entry) {
+        const uint32_t st = ring.slot();
+        if (ring.entry >= S::kRing && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase() ^ 1)) return;
+        const uint32_t dst = ring.addr();
         constexpr int kChunks = S::kUnitPanels * 8;  // 16-byte pieces of a row in this unit
         constexpr int kBatch = 4;
         for (int i0 = tid; i0 < kTile * kChunks; i0 += 96 * kBatch) {
@@ -839,34 +978,32 @@ __device__ void load_role_copy(const ChunkParams &p, uint32_t base, Misc *m) {
               y = make_uint4(T::from_f16x2(h[0]), T::from_f16x2(h[1]), T::from_f16x2(h[2]), T::from_f16x2(h[3]));
             }
             const int row = i / kChunks, c = i % kChunks;
-            const uint32_t to = dst + (c >> 3) * kPanelBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+            const uint32_t to = dst + (c >> 3) * p.panel_stride + (row >> 3) * p.group_stride + (row & 7) * 128 + (((c & 7) ^ (row & 7)) << 4);
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
           }
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&m->kv_full[st]));
-        ring.next<S::kStages>();
-        ++loads;
       }
-      return true;
-    });
-    if (!ok) return;
-    at += stop - w.off;
-    if (at < end) next_tile(p, w);
+    }
+    left -= stop - w.off;
+    if (left > 0) next_tile(p, w);
   }
   if (warp == 0) {
     const uint32_t slot = item % kItems;
-    if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1, gave_up)) return;
+    if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1)) return;
     if (lane == 0) {
       m->items[slot].rows = 0;
       mbar_arrive(smem_addr(&m->item_full[slot]));
     }
   }
-  const uint32_t held = min(loads, static_cast<uint32_t>(S::kStages));  // releases that are still to arrive
-  for (uint32_t k = 0; k < held; ++k) {
-    const uint32_t entry = loads - held + k;
-    if (!warp_wait(smem_addr(&m->kv_empty[entry % S::kStages]), (entry / S::kStages) & 1, gave_up)) return;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {  // releases that are still to arrive
+    Ring<kDp> &ring = rings[k];
+    const uint32_t held = min(ring.entry, static_cast<uint32_t>(S::kRing)), last = ring.entry;
+    for (ring.entry = last - held; ring.entry != last; ++ring.entry)
+      if (!warp_wait(smem_addr(&m->kv_empty[ring.slot()]), ring.phase())) return;
   }
 }
 
@@ -880,139 +1017,133 @@ struct Products {
   static constexpr uint32_t kScores = kTypes | ((kTile >> 3) << 17);
   static constexpr uint32_t kOutput = kTypes | (1u << 16) | ((S::kUnitPanels * 64 / 8) << 17);
 
+  const ChunkParams &p;
+  uint32_t elected;
   uint32_t base, tmem;
   Misc *m;
-  volatile int *gave_up;
-  Ring ring;
-  uint32_t tiles[2] = {0, 0};   // score tiles issued per stream
-  uint32_t weights[2] = {0, 0};  // output products issued per stream
+  Ring<kDp> k_ring, v_ring;
+  uint32_t q_phase = 0, p_phase = 0;  // bit s: parity of the next wait for stream s's queries / weights
+  uint32_t tiles = 0, weights = 0;    // one stream: score tiles and output products issued
+  __device__ __forceinline__ Products(const ChunkParams &params, uint32_t smem_base, uint32_t tmem_base, Misc *misc)
+      : p(params), elected(elect_lane()), base(smem_base), tmem(tmem_base), m(misc), k_ring(smem_base, 0), v_ring(smem_base, 1) {}
 
-  __device__ __forceinline__ bool acquire(Ring *first) {  // one K or V tile
-    *first = ring;
-    for (int u = 0; u < S::kUnits; ++u) {
-      if (!mbar_wait(smem_addr(&m->kv_full[ring.stage]), ring.phase, gave_up)) return false;
-      ring.next<S::kStages>();
-    }
+  __device__ __forceinline__ bool acquire(Ring<kDp> ring) {  // one tile
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u, ++ring.entry)
+      if (!warp_wait(smem_addr(&m->kv_full[ring.slot()]), ring.phase())) return false;
     return true;
   }
-  __device__ __forceinline__ void release(Ring from) {
-    for (int u = 0; u < S::kUnits; ++u) {
-      tc_commit(smem_addr(&m->kv_empty[from.stage]));
-      from.next<S::kStages>();
-    }
+  __device__ __forceinline__ void release(Ring<kDp> &ring) {
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u, ++ring.entry) tc_commit(elected, smem_addr(&m->kv_empty[ring.slot()]));
   }
-  __device__ __forceinline__ void scores(int s, Ring k) {
+  __device__ __forceinline__ void scores(uint32_t s, bool free_q) {
     tc_fence_after();
-    const uint32_t buf = S::kScoreBufs == 2 ? (tiles[s] & 1) : s;
+    const uint32_t buf = S::kScoreBufs == 2 ? (tiles++ & 1) : s;
     const uint32_t d = tmem + buf * kTile;
-    const uint32_t q = base + s * S::kQBytes;
+    Ring<kDp> k = k_ring;
+    uint32_t q = base + s * S::kQBytes;
 #pragma unroll
-    for (int u = 0; u < S::kUnits; ++u) {
-      const uint32_t at = base + S::kRingAt + k.stage * S::kUnitBytes;
+    for (int u = 0; u < S::kUnits; ++u, ++k.entry) {
 #pragma unroll
-      for (int kk = 0; kk < S::kUnitPanels * 4; ++kk) {
-        const uint32_t in = (kk >> 2) * kPanelBytes + (kk & 3) * 32;
-        mma_ss(d, operand_desc(q + u * S::kUnitPanels * kPanelBytes + in, 16, 1024), operand_desc(at + in, 16, 1024), kScores,
-               u > 0 || kk > 0);
+      for (int pp = 0; pp < S::kUnitPanels; ++pp, q += kPanelBytes) {
+        const uint64_t qd = operand_desc(q, 16, 1024);
+        const uint64_t kd = operand_desc(k.addr() + pp * p.panel_stride, 16, p.group_stride);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) mma_ss(elected, d, qd + kk * 2, kd + kk * 2, kScores, u > 0 || pp > 0 || kk > 0);
       }
-      k.next<S::kStages>();
     }
-    tc_commit(smem_addr(&m->s_full[buf]));
-    ++tiles[s];
+    tc_commit(elected, smem_addr(&m->s_full[0]) + 8 * buf);
+    if (free_q) tc_commit(elected, smem_addr(&m->q_empty[0]) + 8 * s);
   }
-  __device__ __forceinline__ bool wait_weights(int s) {
-    const uint32_t buf = S::kScoreBufs == 2 ? (weights[s] & 1) : s;
-    const uint32_t ph = (S::kScoreBufs == 2 ? weights[s] >> 1 : weights[s]) & 1;
-    return mbar_wait(smem_addr(&m->p_full[buf]), ph, gave_up);
-  }
-  __device__ __forceinline__ void output(int s, Ring v, bool first) {
-    tc_fence_after();
-    const uint32_t buf = S::kScoreBufs == 2 ? (weights[s] & 1) : s;
+  // The product over the first three quarters of the tokens runs while the last weights are still
+  // being made.
+  __device__ __forceinline__ bool output(uint32_t s, bool first) {
+    const uint32_t buf = S::kScoreBufs == 2 ? (weights & 1) : s;
+    const uint32_t ph = S::kScoreBufs == 2 ? (weights >> 1 & 1) : (p_phase >> s & 1);
     const uint32_t a = tmem + buf * kTile, d = tmem + 256 + s * kDp;
+    const uint32_t step = p.group_stride >> 3;  // 16 tokens, in descriptor units
+    if (!warp_wait(smem_addr(&m->p_part[0]) + 8 * buf, ph)) return false;
+    tc_fence_after();
+    Ring<kDp> v = v_ring;
 #pragma unroll
-    for (int u = 0; u < S::kUnits; ++u) {
-      const uint32_t at = base + S::kRingAt + v.stage * S::kUnitBytes;
+    for (int u = 0; u < S::kUnits; ++u, ++v.entry) {
+      const uint64_t vd = operand_desc(v.addr(), p.panel_stride, p.group_stride);
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk)
-        mma_ts(d + u * 128, a + kk * 8, operand_desc(at + kk * 2048, kPanelBytes, 1024), kOutput, !first || kk > 0);
-      v.next<S::kStages>();
+      for (int kk = 0; kk < 6; ++kk) mma_ts(elected, d + u * 128, a + kk * 8, vd + kk * step, kOutput, !first || kk > 0);
     }
-    tc_commit(smem_addr(&m->pv_done[s]));
-    ++weights[s];
+    if (!warp_wait(smem_addr(&m->p_full[0]) + 8 * buf, ph)) return false;
+    tc_fence_after();
+    v = v_ring;
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u, ++v.entry) {
+      const uint64_t vd = operand_desc(v.addr(), p.panel_stride, p.group_stride);
+#pragma unroll
+      for (int kk = 6; kk < 8; ++kk) mma_ts(elected, d + u * 128, a + kk * 8, vd + kk * step, kOutput, 1);
+    }
+    tc_commit(elected, smem_addr(&m->pv_done[0]) + 8 * s);
+    p_phase ^= 1u << s;
+    ++weights;
+    return true;
   }
 
-  __device__ bool piece(const ChunkParams &p, const Piece &x, uint32_t *queries) {
-    int b[2] = {0, 0}, e[2] = {0, 0};
+  __device__ __forceinline__ bool piece(const Piece &x) {
+    int n0 = 0, n1 = 0;
+#pragma unroll
     for (int s = 0; s < S::kStreams; ++s) {
-      stream_range<S::kStreams>(p, x, s, &b[s], &e[s]);
-      if (e[s] > b[s] && !mbar_wait(smem_addr(&m->q_full[s]), queries[s]++ & 1, gave_up)) return false;
+      int b, e;
+      stream_range<S::kStreams>(p, x, s, &b, &e);
+      const int n = __reduce_max_sync(0xFFFFFFFFu, e - b);  // (uniform, and known to be)
+      if (s == 0)
+        n0 = n;
+      else
+        n1 = n;
+      if (n == 0) continue;
+      if (!warp_wait(smem_addr(&m->q_full[s]), q_phase >> s & 1)) return false;
+      q_phase ^= 1u << s;
     }
-    const int n0 = e[0] - b[0], n1 = e[1] - b[1];
-    Ring k, v;
-    if (S::kStreams == 1) {
-      if (n0 > 0) {
-        if (!acquire(&k)) return false;
-        scores(0, k);
-        release(k);
-      }
-      for (int i = 0; i < n0; ++i) {
-        if (i + 1 < n0) {
-          if (!acquire(&k)) return false;
-          scores(0, k);
-          release(k);
+    // the query tile of stream 1 is the join's buffer first
+    const bool joins = __any_sync(0xFFFFFFFFu, joins_streams(x)) != 0;
+    const bool narrow = S::kStreams == 2 && __any_sync(0xFFFFFFFFu, x.narrow) != 0;
+    const int most = max(n0, n1);
+    if (most == 0) return true;
+#pragma unroll 1
+    for (int i = 0; i <= most; ++i) {
+      if (S::kStreams == 1) {  // scores of the next tile ahead of the output product of this one
+        if (i < most) {
+          if (!acquire(k_ring)) return false;
+          scores(0, p.q_tma && i + 1 == most);
+          release(k_ring);
         }
-        if (!wait_weights(0) || !acquire(&v)) return false;
-        output(0, v, i == 0);
-        release(v);
-      }
-      return true;
-    }
-    if (x.narrow) {
-      for (int s = 0; s < 2; ++s) {
-        if (e[s] == b[s]) continue;
-        if (!acquire(&k)) return false;
-        scores(s, k);
-        release(k);
-      }
-      for (int i = 0; i < n0; ++i) {
-        for (int s = 0; s < 2; ++s) {
-          const int n = s == 0 ? n0 : n1;
-          if (i >= n) continue;
-          if (!wait_weights(s) || !acquire(&v)) return false;
-          output(s, v, i == 0);
-          release(v);
-          if (i + 1 < n) {
-            if (!acquire(&k)) return false;
-            scores(s, k);
-            release(k);
-          }
+        if (i > 0) {
+          if (!acquire(v_ring) || !output(0, i == 1)) return false;
+          release(v_ring);
         }
+        continue;
       }
-      return true;
-    }
-    const int n = max(n0, n1);
-    if (n > 0) {
-      if (!acquire(&k)) return false;
-      if (n0 > 0) scores(0, k);
-      if (n1 > 0) scores(1, k);
-      release(k);
-    }
-    for (int i = 0; i < n; ++i) {
-      if (i < n0 && !wait_weights(0)) return false;
-      if (!acquire(&v)) return false;
-      if (i < n0) output(0, v, i == 0);
-      if (i + 1 < n) {
-        if (!acquire(&k)) return false;
-        if (i + 1 < n0) scores(0, k);
-      }
-      if (i < n1) {
-        if (!wait_weights(1)) return false;
-        output(1, v, i == 0);
-      }
-      release(v);
-      if (i + 1 < n) {
-        if (i + 1 < n1) scores(1, k);
-        release(k);
+      bool has_k = false, has_v = false;
+#pragma unroll 1
+      for (uint32_t s = 0; s < 2; ++s) {
+        const int n = s == 0 ? n0 : n1;
+        const bool done = narrow || s == 1;  // the tile's last reader
+        if (i > 0 && i <= n) {
+          if (!has_v && !acquire(v_ring)) return false;
+          has_v = true;
+          if (!output(s, i == 1)) return false;
+        }
+        if (has_v && done) {
+          release(v_ring);
+          has_v = false;
+        }
+        if (i < n) {
+          if (!has_k && !acquire(k_ring)) return false;
+          has_k = true;
+          scores(s, p.q_tma && i + 1 == n && !(s == 1 && joins));
+        }
+        if (has_k && done) {
+          release(k_ring);
+          has_k = false;
+        }
       }
     }
     return true;
@@ -1026,53 +1157,107 @@ struct Products {
 // sums in tensor memory are rescaled on a few tiles instead of on every one.
 constexpr float kLazy = 8.f;
 
-// One row of a piece again, token by token and only those it may see.  A masked token has weight
-// zero in the products, but zero times an infinity or a NaN that its V holds is a NaN: a row that
-// comes out of the products not finite although tokens were masked for it is redone here.
+#ifndef KVX_CHUNK_POLY
+#define KVX_CHUNK_POLY 2  // pairs of 8 whose exponentials are made by exp2_pair
+#endif
+
+// 2^z on the f32 pipes, for a pair: the exponent unit alone (16 results per clock and SM) would be
+// what bounds the kernel.  z = n + f with n the nearest integer (its bits appear in the low end of
+// z + kRound); 2^f by a polynomial of degree 4 on [-1/2, 1/2], fitted for the least relative error
+// (2^-18.5, well below the 2^-9 or 2^-12 that rounding a weight costs); times the float whose
+// exponent field is n + 127.  z is held at -127 or above, where that field, and the result, is zero;
+// a NaN stays one.
+__device__ __forceinline__ float2 exp2_pair(float2 z) {
+  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23, and the exponent bias
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.y) : "f"(-127.f));
+  const float2 r = __fadd2_rn(z, make_float2(kRound, kRound));
+  const float2 n = __fadd2_rn(r, make_float2(-kRound, -kRound));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), z);
+  float2 y = __ffma2_rn(make_float2(0.00957053154706955f, 0.00957053154706955f), f, make_float2(0.05591866374015808f, 0.05591866374015808f));
+  y = __ffma2_rn(y, f, make_float2(0.24024735391139984f, 0.24024735391139984f));
+  y = __ffma2_rn(y, f, make_float2(0.6931216716766357f, 0.6931216716766357f));
+  y = __ffma2_rn(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return __fmul2_rn(y, make_float2(__uint_as_float(__float_as_uint(r.x) << 23), __uint_as_float(__float_as_uint(r.y) << 23)));
+}
+
+// Weights of 16 scores of one row: exponentials, their sum, and the rounded pairs to tensor memory.
+template <typename T>
+__device__ __forceinline__ void weigh(const float *sc, float2 mul2, float2 sub2, float2 &sum2, uint32_t to) {
+  uint32_t w[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float2 z = __ffma2_rn(make_float2(sc[2 * k], sc[2 * k + 1]), mul2, sub2);
+    const bool poly = (k + 1) * KVX_CHUNK_POLY / 8 != k * KVX_CHUNK_POLY / 8;  // spread evenly
+    const float2 y = poly ? exp2_pair(z) : make_float2(fast_exp2(z.x), fast_exp2(z.y));
+    sum2 = __fadd2_rn(sum2, y);
+    w[k] = T::pack2(y.x, y.y);
+  }
+  tc_st8(to, w);
+}
+
+// Whether the page of this lane's four tokens of the tile at `first` exists; page sizes that are not a
+// multiple of four are looked up token by token where it matters.
+__device__ __forceinline__ bool pages_exist(const ChunkParams &p, const Piece &x, int32_t first) {
+  const int32_t tok = first + (threadIdx.x & 31) * 4;
+  return tok >= x.q.len || ((p.block_size & 3) == 0 && page_of(p, x.seq, tok) >= 0);
+}
+
+// One row of a piece again, token by token and only those it may see, under the maximum `mx` its
+// weights were made with.  A masked token has weight zero in the products, but zero times an
+// infinity or a NaN that its V holds is a NaN: a row that comes out of the products not finite
+// although tokens were masked for it is redone here.
 template <int kDp>
-__device__ void redo_row(const ChunkParams &p, const Piece &x, int32_t r, float mul, float *o, float *m_out, float *l_out) {
+__device__ __noinline__ void redo_row(const ChunkParams &p, const Piece &x, int32_t r, float mul, float mx, float *o) {
   const int lane = threadIdx.x & 31;
   constexpr int kPer = kDp / 32;
   const int32_t token = r / p.group, qh = x.head * p.group + r % p.group;
   const char *q = p.query + (x.q.first + token) * p.q_pitch + static_cast<int64_t>(qh) * p.dim * 2;
-  float qv[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int d = lane + 32 * i;
-    qv[i] = d < p.dim ? load_f32(q + d * 2, p.io_code) : 0.f;
-    if (mul < 0.f) qv[i] = -qv[i];
-    if (mul == 0.f) qv[i] = 0.f;
-    o[i] = 0.f;
-  }
-  const float am = score_abs(mul);
-  float m = -INFINITY, l = 0.f;
+  const float sub = mx == -INFINITY ? 0.f : -mx * fabsf(mul);
+#pragma unroll 1
+  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
   const int32_t end = min(row_limit(p, x.q, r), x.kv1 * kTile);
+#pragma unroll 1
   for (int32_t t = x.kv0 * kTile; t < end; ++t) {
     const int32_t page = page_of(p, x.seq, t);
     if (page < 0) continue;
     const int32_t at = t % p.block_size;
     const char *kp = p.k.base + page * p.k.blk, *vp = p.v.base + page * p.v.blk;
     float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 32 * i;
-      if (d < p.dim) dot = fmaf(qv[i], load_f32(kp + head_offset(p.k, at, x.head, d), p.cache_code), dot);
-    }
+#pragma unroll 1
+    for (int d = lane; d < p.dim; d += 32)
+      dot = fmaf(load_f32(q + d * 2, p.io_code), load_f32(kp + head_offset(p.k, at, x.head, d), p.cache_code), dot);
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, s);
-    const float mn = fmaxf(m, dot);
-    const float c = weight_of(m, mn, am);
-    const float w = mn == -INFINITY ? (dot == dot ? 0.f : dot) : exp2f((dot - mn) * am);
-    l = l * c + w;
-#pragma unroll
+    const float w = exp2f(fmaf(dot, mul, sub));
+#pragma unroll 1
     for (int i = 0; i < kPer; ++i) {
       const int d = lane + 32 * i;
-      const float vv = d < p.dim ? load_f32(vp + head_offset(p.v, at, x.head, d), p.cache_code) : 0.f;
-      o[i] = o[i] * c + (w == 0.f ? 0.f * vv : w * vv);
+      if (d < p.dim) o[i] = fmaf(w, load_f32(vp + head_offset(p.v, at, x.head, d), p.cache_code), o[i]);
     }
-    m = mn;
   }
-  *m_out = m, *l_out = l;
+}
+
+// Sets scores that must not count (tokens the row may not see, tokens without a page) to -inf, and
+// gives the others the sign of the multiplier.
+__device__ __forceinline__ void correct_scores(const ChunkParams &p, const Piece &x, uint32_t s_at, int32_t first, int32_t valid, bool gaps,
+                                               float sign) {
+#pragma unroll 1
+  for (int k = 0; k < kTile; k += 32) {
+    float c[32];
+    tc_ld32(c, s_at + k);
+    unsigned has = 0xFFFFFFFFu;
+    if (gaps) {
+      const int32_t tok = first + k + (threadIdx.x & 31);
+      has = __ballot_sync(0xFFFFFFFFu, tok >= x.q.len || page_of(p, x.seq, tok) >= 0);
+    }
+    if (valid - k < 32) has &= valid <= k ? 0u : (1u << (valid - k)) - 1;
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) c[i] = (has >> i) & 1 ? c[i] * sign : -INFINITY;
+    tc_st32(s_at + k, c);
+  }
+  tc_wait_st();
 }
 
 template <typename T, int kDp>
@@ -1081,12 +1266,12 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
   const int s = threadIdx.x >> 7;                 // stream
   const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
   const uint32_t lanes = static_cast<uint32_t>((tid >> 5) * 32) << 16;  // this warp's lanes of tensor memory
-  volatile int *gave_up = &m->gave_up;
-  uint32_t tiles = 0;       // score tiles of this stream so far
+  uint32_t tiles = 0;  // score tiles of this stream so far
   uint32_t joins = 0;
+#pragma unroll 1
   for (uint32_t item = 0;; ++item) {
     const uint32_t slot = item % kItems;
-    if (!warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1, gave_up)) return;
+    if (!warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1)) return;
     const Piece x = m->items[slot];
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_addr(&m->item_empty[slot]));
@@ -1097,84 +1282,80 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
     const int32_t row_at = x.row0 + (narrow ? 0 : s * kTile);   // first group row of this stream
     const int32_t rows = min(kTile, x.rows - (narrow ? 0 : s * kTile));
     if (rows <= 0) continue;
-    const float mul = score_mul(p, x.head);
-    const float am = score_abs(mul);
+    const float mul = nonzero(score_mul(p, x.head));
+    const float am = fabsf(mul), sign = mul > 0.f ? 1.f : -1.f;
 
-    if (e > b) {
+    if (e > b && !p.q_tma) {
       // Query rows into the swizzled operand tile (its last reader, the scores of this stream's
       // previous tile, was waited for).
-      const uint32_t flip = mul < 0.f ? 0x80008000u : 0u, keep = mul == 0.f ? 0u : 0xFFFFFFFFu;
-      constexpr int kChunks = kDp / 8;
-      for (int i = tid; i < kTile * kChunks; i += 128) {
-        const int row = i / kChunks, c = i % kChunks, d = c * 8;
-        uint4 y = make_uint4(0, 0, 0, 0);
-        if (row < rows && d < p.dim) {
-          const int32_t r = row_at + row, token = r / p.group, h = x.head * p.group + (r - token * p.group);
-          const char *src = p.query + (x.q.first + token) * p.q_pitch + (static_cast<int64_t>(h) * p.dim + d) * 2;
-          if (p.q_vec) {
-            y = *reinterpret_cast<const uint4 *>(src);
-          } else {
-            uint16_t t[8];
+      constexpr int kChunks = kDp / 8, kBatch = 4;
+#pragma unroll 1
+      for (int i0 = tid; i0 < kTile * kChunks; i0 += 128 * kBatch) {
+        uint4 y[kBatch];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[k] = d + k < p.dim ? reinterpret_cast<const uint16_t *>(src)[k] : 0;
-            y = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = i0 + 128 * k, row = i / kChunks, d = i % kChunks * 8;
+          y[k] = make_uint4(0, 0, 0, 0);
+          if (row < rows && d < p.dim) {
+            const int32_t r = row_at + row, token = r / p.group, hq = x.head * p.group + (r - token * p.group);
+            const char *src = p.query + (x.q.first + token) * p.q_pitch + (static_cast<int64_t>(hq) * p.dim + d) * 2;
+            if (p.q_vec) {
+              y[k] = *reinterpret_cast<const uint4 *>(src);
+            } else {
+              uint32_t t[4] = {0, 0, 0, 0};
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                if (d + c < p.dim) t[c >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(src)[c]) << ((c & 1) * 16);
+              y[k] = make_uint4(t[0], t[1], t[2], t[3]);
+            }
           }
-          y.x = (y.x ^ flip) & keep, y.y = (y.y ^ flip) & keep, y.z = (y.z ^ flip) & keep, y.w = (y.w ^ flip) & keep;
         }
-        const uint32_t to = base + s * S::kQBytes + (c >> 3) * kPanelBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = i0 + 128 * k, row = i / kChunks, c = i % kChunks;
+          const uint32_t to = base + s * S::kQBytes + (c >> 3) * kPanelBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(y[k].x), "r"(y[k].y), "r"(y[k].z), "r"(y[k].w) : "memory");
+        }
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&m->q_full[s]));
+      if (lane == 0) mbar_arrive(smem_addr(&m->q_full[0]) + 8 * s);
     }
 
     // (rows behind the tile's last are never written: nothing is masked for them)
     const int32_t limit = tid < rows ? row_limit(p, x.q, row_at + tid) : INT32_MAX;
     float mx = -INFINITY, l = 0.f;
     const uint32_t o_at = tmem0 + lanes + 256 + s * kDp;
+    bool page_ok = pages_exist(p, x, b * kTile);
+#pragma unroll 1
     for (int j = b; j < e; ++j, ++tiles) {
       const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
       const uint32_t ph = (S::kScoreBufs == 2 ? tiles >> 1 : tiles) & 1;
       const uint32_t s_at = tmem0 + lanes + buf * kTile;
-      // does every page of the tile exist?  four tokens per lane (page sizes that are not a
-      // multiple of four are looked up token by token below)
-      int32_t page_ok = 1;
-      {
-        const int32_t tok = j * kTile + lane * 4;
-        if (tok < x.q.len) page_ok = (p.block_size & 3) == 0 && page_of(p, x.seq, tok) >= 0;
-      }
       const int32_t valid = limit == INT32_MAX ? kTile : min(kTile, limit - j * kTile);  // visible tokens of this row (may be negative)
-      const bool masked = __any_sync(0xFFFFFFFFu, valid < kTile) != 0;
-      const bool holes = __all_sync(0xFFFFFFFFu, page_ok) == 0;
-      if (!warp_wait(smem_addr(&m->s_full[buf]), ph, gave_up)) return;
+      const bool plain = __all_sync(0xFFFFFFFFu, valid == kTile && page_ok && mul > 0.f) != 0;
+      const bool gaps = __all_sync(0xFFFFFFFFu, page_ok) == 0;
+      if (!warp_wait(smem_addr(&m->s_full[0]) + 8 * buf, ph)) return;
       tc_fence_after();
-      float sc[kTile];
+      if (!plain) correct_scores(p, x, s_at, j * kTile, valid, gaps, sign);
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int k = 0; k < kTile; k += 64) {
+        float c0[32], c1[32];
+        tc_ld32(c0, s_at + k);
+        tc_ld32(c1, s_at + k + 32);
+        tc_wait_ld();
+        float t0 = top, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tc_ld32(sc + 32 * c, s_at + 32 * c);
-      tc_wait_ld();
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < kTile; ++c)
-          if (c >= valid) sc[c] = -INFINITY;
-      }
-      if (holes) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int32_t tok = j * kTile + c * 32 + lane;
-          const unsigned has = __ballot_sync(0xFFFFFFFFu, tok >= x.q.len || page_of(p, x.seq, tok) >= 0);
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (!((has >> k) & 1)) sc[32 * c + k] = -INFINITY;
+        for (int i = 0; i < 32; i += 4) {
+          t0 = fmaxf(fmaxf(t0, c0[i]), c0[i + 1]);
+          t1 = fmaxf(fmaxf(t1, c1[i]), c1[i + 1]);
+          t2 = fmaxf(fmaxf(t2, c0[i + 2]), c0[i + 3]);
+          t3 = fmaxf(fmaxf(t3, c1[i + 2]), c1[i + 3]);
         }
+        top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
       }
-      float t0 = fmaxf(sc[0], sc[1]), t1 = fmaxf(sc[2], sc[3]);
-#pragma unroll
-      for (int c = 4; c < kTile; c += 4) {
-        t0 = fmaxf(fmaxf(t0, sc[c]), sc[c + 1]);
-        t1 = fmaxf(fmaxf(t1, sc[c + 2]), sc[c + 3]);
-      }
-      const float top = fmaxf(t0, t1);
+      page_ok = pages_exist(p, x, (j + 1) * kTile);  // of the next tile: on its way meanwhile
       const bool raise = top > mx && (mx == -INFINITY || (top - mx) * am > kLazy);
       if (__any_sync(0xFFFFFFFFu, raise)) {
         const float c = raise ? weight_of(mx, top, am) : 1.f;
@@ -1182,88 +1363,95 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
         if (j > b) {
           l *= c;
           // the sums of the tiles so far must be complete before they are rescaled
-          if (!warp_wait(smem_addr(&m->pv_done[s]), (tiles - 1) & 1, gave_up)) return;
+          if (!warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (tiles - 1) & 1)) return;
           tc_fence_after();
 #pragma unroll 1
-          for (int k = 0; k < kDp / 16; ++k) {
-            uint32_t o[16];
-            tc_ld16(o, o_at + 16 * k);
+          for (int k = 0; k < kDp; k += 16) {
+            float o[16];
+            tc_ld16(o, o_at + k);
             tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
-            tc_st16(o_at + 16 * k, o);
+            for (int i = 0; i < 16; ++i) o[i] *= c;
+            tc_st16(o_at + k, reinterpret_cast<const uint32_t *>(o));
           }
         }
       }
       // weights exp2((score - mx) * am); a row that has seen no token yet subtracts 0
       const float sub = mx == -INFINITY ? 0.f : -mx * am;
-      const float2 am2 = make_float2(am, am), sub2 = make_float2(sub, sub);
+      const float2 mul2 = make_float2(am, am), sub2 = make_float2(sub, sub);
       float2 sum2 = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 z = __ffma2_rn(make_float2(sc[32 * c + 2 * k], sc[32 * c + 2 * k + 1]), am2, sub2);
-          const float2 y = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-          sum2 = __fadd2_rn(sum2, y);
-          w[k] = T::pack2(y.x, y.y);
+      {
+        // 16 columns at a time, the next 16 on their way; the weights of columns c, c + 1 go to column
+        // c / 2, which has been read by then.
+        float c0[16], c1[16];
+        tc_ld16(c0, s_at);
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          tc_wait_ld();
+          tc_ld16(c1, s_at + 32 * k + 16);
+          if (k == 3) {
+            // Three quarters are made.  One stream: the scores of this tile were issued ahead of the
+            // previous output product, so they do not tell that it has ended.  Weights are handed over
+            // only after it has -- its barrier is then never more than one phase away from the
+            // parity that is waited for.
+            if (S::kScoreBufs == 2 && j > b && !warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (tiles - 1) & 1)) return;
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_addr(&m->p_part[0]) + 8 * buf);
+          }
+          weigh<T>(c0, mul2, sub2, sum2, s_at + 16 * k);
+          tc_wait_ld();
+          if (k < 3) tc_ld16(c0, s_at + 32 * k + 32);
+          weigh<T>(c1, mul2, sub2, sum2, s_at + 16 * k + 8);
         }
-        tc_st16(s_at + 16 * c, w);
       }
       l += sum2.x + sum2.y;
       tc_wait_st();
-      // One stream: the scores of this tile were issued ahead of the previous output product, so they
-      // do not tell that it has ended.  Weights are handed over only after it has -- the barrier is
-      // then never more than one phase away from the parity that is waited for.
-      if (S::kScoreBufs == 2 && j > b && !warp_wait(smem_addr(&m->pv_done[s]), (tiles - 1) & 1, gave_up)) return;
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&m->p_full[buf]));
+      if (lane == 0) mbar_arrive(smem_addr(&m->p_full[0]) + 8 * buf);
     }
 
+    // ---- the piece's result ----
     if (e > b) {
-      if (!warp_wait(smem_addr(&m->pv_done[s]), (tiles - 1) & 1, gave_up)) return;
+      if (!warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (tiles - 1) & 1)) return;
       tc_fence_after();
     }
-    // ---- the piece's result ----
     const float vmul = p.vs.base != nullptr ? p.vs.base[x.head * p.vs.stride] : 1.f;
-    float f_own = 1.f, f_other = 0.f;
-    const bool join = narrow && x.kv1 - x.kv0 > 1;  // stream 1 has tiles of its own
-    if (join) {
-      if (s == 1) {
-        // hand sums, maximum and denominator to stream 0 through this stream's query tile
-        m->join_m[tid] = mx, m->join_l[tid] = l;
-        float *buf = reinterpret_cast<float *>(smem + S::kQBytes);  // [kDp / 2][128]
+    const bool join = S::kStreams == 2 && joins_streams(x);
+    // Stream 1 hands its sums to stream 0 through its query tile, [kDp / 2][128] at a time.
+    float *joint = reinterpret_cast<float *>(smem + S::kQBytes) + tid;
+    if (narrow && s == 1) {
+      if (!join) continue;
+      m->join_m[tid] = mx, m->join_l[tid] = l;
+#pragma unroll 1
+      for (int k = 0; k < kDp; k += 16) {
+        if (k == kDp / 2) {
+          if (!warp_wait(smem_addr(&m->join_empty), joins & 1)) return;
+          ++joins;
+        }
+        float o[16];
+        tc_ld16(o, o_at + k);
+        tc_wait_ld();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half == 1) {
-            if (!warp_wait(smem_addr(&m->join_empty), joins & 1, gave_up)) return;
-            ++joins;
-          }
-#pragma unroll
-          for (int k = 0; k < kDp / 64; ++k) {
-            float o[32];
-            tc_ld32(o, o_at + half * (kDp / 2) + 32 * k);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) buf[(32 * k + i) * kTile + tid] = o[i];
-          }
+        for (int i = 0; i < 16; ++i) joint[(k % (kDp / 2) + i) * kTile] = o[i];
+        if (k % (kDp / 2) + 16 == kDp / 2) {
+          fence_async_smem();  // TMA may fill the tile next
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_addr(&m->join_full));
         }
-        // the query tile is free again once stream 0 has read the second half
-        if (!warp_wait(smem_addr(&m->join_empty), joins & 1, gave_up)) return;
-        ++joins;
-        tc_fence_before();
-        continue;
       }
-    } else if (narrow && s == 1) {
+      // the query tile is free again once stream 0 has read the second part
+      if (!warp_wait(smem_addr(&m->join_empty), joins & 1)) return;
+      ++joins;
+      if (p.q_tma && tid == 0) mbar_arrive(smem_addr(&m->q_empty[1]));
+      tc_fence_before();
       continue;
     }
-    uint32_t join_at = joins;
+    float f_own = 1.f, f_other = 0.f;
     if (join) {
-      if (!warp_wait(smem_addr(&m->join_full), join_at & 1, gave_up)) return;
+      if (!warp_wait(smem_addr(&m->join_full), joins & 1)) return;
       const float m1 = m->join_m[tid], l1 = m->join_l[tid];
       const float top = fmaxf(mx, m1);
       f_own = weight_of(mx, top, am), f_other = weight_of(m1, top, am);
@@ -1272,55 +1460,87 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
     }
     const int32_t r = row_at + tid;
     const int32_t token = r / p.group, qh = x.head * p.group + r % p.group;
-    const float *joined = reinterpret_cast<const float *>(smem + S::kQBytes);
     char *out = p.out + (x.q.first + token) * p.o_pitch + static_cast<int64_t>(qh) * p.dim * 2;
     const int64_t part = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + (r - x.row0);
     const float mul_out = l == 0.f ? 0.f : (x.slot < 0 ? vmul / l : vmul);
-    float finite = 0.f;
+    float finite = 0.f;  // becomes NaN with the first value that is not finite
     const bool vec_out = p.q_vec != 0;
+    char *quad_out[4];  // the rows of this thread and its three neighbours
 #pragma unroll
-    for (int k = 0; k < kDp / 32; ++k) {
-      if (join && k == kDp / 64) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&m->join_empty));
-        if (!warp_wait(smem_addr(&m->join_full), (join_at + 1) & 1, gave_up)) return;
-      }
+    for (int c = 0; c < 4; ++c)
+      quad_out[c] = reinterpret_cast<char *>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(out), (lane & ~3) + c));
+#pragma unroll 1
+    for (int k = 0; k < kDp; k += 32) {
+      const int d0 = k;
       float o[32];
       if (e > b) {
-        tc_ld32(o, o_at + 32 * k);
+        tc_ld32(o, o_at + k);
         tc_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+      }
+      if (join) {
+        if (k == kDp / 2) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&m->join_empty));
+          if (!warp_wait(smem_addr(&m->join_full), (joins + 1) & 1)) return;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = o[i] * f_own + joint[(k % (kDp / 2) + i) * kTile] * f_other;
       }
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        float y = e > b ? o[i] : 0.f;
-        if (join) y = y * f_own + joined[((k % (kDp / 64)) * 32 + i) * kTile + tid] * f_other;
-        y *= mul_out;
-        if (l == 0.f) y = 0.f;
-        finite = fmaf(y, 0.f, finite);  // NaN as soon as one value is not finite
-        o[i] = y;
+        o[i] = l == 0.f ? 0.f : o[i] * mul_out;
+        finite = fmaf(o[i], 0.f, finite);
       }
-      if (tid < rows) {
+      if (x.slot < 0 && vec_out) {
+        // A thread has 64 bytes of its row; four threads exchange 16-byte pieces so that each store
+        // instruction writes 64 bytes of 8 rows instead of 16 bytes of 32.
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = T::pack2(o[2 * i], o[2 * i + 1]);
+#pragma unroll
+        for (int bit = 1; bit <= 2; bit <<= 1) {
+          const bool up = (lane & bit) != 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c & bit) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? w[4 * c + i] : w[4 * (c | bit) + i], bit);
+              if (up)
+                w[4 * c + i] = got;
+              else
+                w[4 * (c | bit) + i] = got;
+            }
+          }
+        }
+        const int d = d0 + (lane & 3) * 8;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if ((tid & ~3) + c < rows && d < p.dim)
+            *reinterpret_cast<uint4 *>(quad_out[c] + d * 2) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+      } else if (tid < rows) {
         if (x.slot >= 0) {
-          float *to = p.part_o + part * p.dim + 32 * k;
+          float *to = p.part_o + part * p.dim + d0;
           if ((p.dim & 3) == 0) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
-              if (32 * k + i < p.dim) *reinterpret_cast<float4 *>(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              if (d0 + i < p.dim) *reinterpret_cast<float4 *>(to + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (32 * k + i < p.dim) to[i] = o[i];
+              if (d0 + i < p.dim) to[i] = o[i];
           }
-        } else if (vec_out) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (32 * k + i < p.dim)
-              *reinterpret_cast<uint4 *>(out + (32 * k + i) * 2) =
-                  make_uint4(T::pack2(o[i], o[i + 1]), T::pack2(o[i + 2], o[i + 3]), T::pack2(o[i + 4], o[i + 5]), T::pack2(o[i + 6], o[i + 7]));
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * k + i < p.dim) store_f32(out, 32 * k + i, o[i], p.io_code);
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t w = T::pack2(o[2 * i], o[2 * i + 1]);
+            uint16_t *to = reinterpret_cast<uint16_t *>(out) + d0 + 2 * i;
+            if (d0 + 2 * i < p.dim) to[0] = static_cast<uint16_t>(w);
+            if (d0 + 2 * i + 1 < p.dim) to[1] = static_cast<uint16_t>(w >> 16);
+          }
         }
       }
     }
@@ -1337,30 +1557,36 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
       const int from = __ffs(again) - 1;
       again &= again - 1;
       const int32_t rr = row_at + (tid & ~31) + from;
-      float o[kDp / 32], m2, l2;
-      redo_row<kDp>(p, x, rr, mul, o, &m2, &l2);
-      const float f = l2 == 0.f ? 0.f : (x.slot < 0 ? vmul / l2 : vmul);
+      float o[kDp / 32];
+      const Piece y = x;  // (a copy: the reference keeps it in memory)
+      redo_row<kDp>(p, y, rr, mul, __shfl_sync(0xFFFFFFFFu, mx, from), o);
+      const float f = __shfl_sync(0xFFFFFFFFu, mul_out, from);
       const int32_t tk = rr / p.group, hh = x.head * p.group + rr % p.group;
       char *to = p.out + (x.q.first + tk) * p.o_pitch + static_cast<int64_t>(hh) * p.dim * 2;
       const int64_t slot_row = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + (rr - x.row0);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < kDp / 32; ++i) {
         const int d = lane + 32 * i;
         if (d >= p.dim) continue;
-        const float y = l2 == 0.f ? 0.f : o[i] * f;
         if (x.slot >= 0)
-          p.part_o[slot_row * p.dim + d] = y;
+          p.part_o[slot_row * p.dim + d] = o[i] * f;
         else
-          store_f32(to, d, y, p.io_code);
+          store_f32(to, d, o[i] * f, p.io_code);
       }
-      if (x.slot >= 0 && lane == 0) reinterpret_cast<float2 *>(p.part_ml)[slot_row] = make_float2(m2, l2);
     }
   }
 }
 
+// The kernel's code size is part of its speed: warps of five roles run different code at the same
+// time, and straight-line code that is not in the instruction caches runs at about 8 clocks an
+// instruction.  Loops over columns are therefore kept as loops of 32 to 64 columns, every role has
+// one call site per large routine, and branches on the stream number are avoided (the compiler
+// would clone the loop per stream).  266 KB of code against 60 KB: 1.82 against 1.3 ms for 16 prompts
+// of 512 to 4096 tokens.
 template <typename T, int kDp, bool kTma>
 __global__ void __launch_bounds__(kThreads, 1)
-    kvx_chunk_attention_kernel(const ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    kvx_chunk_attention_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                               const __grid_constant__ CUtensorMap qmap) {
   using S = Shape<kDp>;
   extern __shared__ char smem_raw[];
   char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -1371,26 +1597,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kItems; ++i) {
       mbar_init(smem_addr(&m->item_full[i]), 1);
-      mbar_init(smem_addr(&m->item_empty[i]), S::kStreams * 4 + 1);  // softmax warps and the issuing thread
+      mbar_init(smem_addr(&m->item_empty[i]), S::kStreams * 4 + (kTma ? 2 : 1));  // softmax warps, products, V loads
     }
-    for (int i = 0; i < S::kStages; ++i) {
+    for (int i = 0; i < 2 * S::kRing; ++i) {
       mbar_init(smem_addr(&m->kv_full[i]), kTma ? 1 : 3);
       mbar_init(smem_addr(&m->kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&m->q_full[i]), 4);
+      mbar_init(smem_addr(&m->q_full[i]), p.q_tma ? 1 : 4);
+      mbar_init(smem_addr(&m->q_empty[i]), 1);
       mbar_init(smem_addr(&m->s_full[i]), 1);
+      mbar_init(smem_addr(&m->p_part[i]), 4);
       mbar_init(smem_addr(&m->p_full[i]), 4);
       mbar_init(smem_addr(&m->pv_done[i]), 1);
     }
-    mbar_init(smem_addr(&m->tail), 1);
-    mbar_init(smem_addr(&m->drain), 1);
     mbar_init(smem_addr(&m->join_full), 4);
     mbar_init(smem_addr(&m->join_empty), 4);
-    m->gave_up = 0;
+    mbar_init(smem_addr(&m->tail), 1);
+    mbar_init(smem_addr(&m->drain), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&m->tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -1400,39 +1627,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = m->tmem;
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    if ((warp >> 2) < S::kStreams) softmax_role<T, kDp>(p, base, smem, tmem, m);
+  if (warp < kMmaWarp) {
+    if (S::kStreams == 2 || warp < 4) softmax_role<T, kDp>(p, base, smem, tmem, m);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
-      if ((threadIdx.x & 31) == 0) {
-        Products<T, kDp> pr;
-        pr.base = base, pr.tmem = tmem, pr.m = m, pr.gave_up = &m->gave_up;
-        uint32_t queries[2] = {0, 0};
-        for (uint32_t item = 0;; ++item) {
-          const uint32_t slot = item % kItems;
-          if (!mbar_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1, &m->gave_up)) break;
-          const Piece x = m->items[slot];
-          mbar_arrive(smem_addr(&m->item_empty[slot]));
-          if (x.rows == 0 || !pr.piece(p, x, queries)) break;
-        }
-        // every product has ended before tensor memory is given back
-        tc_commit(smem_addr(&m->drain));
-        int never = 0;
-        mbar_wait(smem_addr(&m->drain), 0, &never);
+    if (warp == kMmaWarp) {
+      Products<T, kDp> pr(p, base, __reduce_max_sync(0xFFFFFFFFu, tmem), m);
+#pragma unroll 1
+      for (uint32_t item = 0;; ++item) {
+        const uint32_t slot = item % kItems;
+        if (!warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1)) break;
+        const Piece x = m->items[slot];
+        __syncwarp();
+        if (pr.elected) mbar_arrive(smem_addr(&m->item_empty[slot]));
+        __syncwarp();
+        if (__all_sync(0xFFFFFFFFu, x.rows == 0) || !pr.piece(x)) break;
       }
+      // every product has ended before tensor memory is given back
+      tc_commit(pr.elected, smem_addr(&m->drain));
+      mbar_wait(smem_addr(&m->drain), 0);
       __syncwarp();
     } else if (kTma) {
-      if (warp == 9) load_role_tma<kDp>(p, &kmap, &vmap, base, m);
+      if (warp <= kMmaWarp + 2) load_role_tma<kDp>(p, &kmap, &vmap, &qmap, base, m, warp == kMmaWarp + 2);
     } else {
-      load_role_copy<T, kDp>(p, base, m);
+      load_role_copy<T, kDp>(p, &qmap, base, m);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // ------------------------------------------------------------------ f32 and everything else --
@@ -1457,17 +1680,15 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
   int32_t *sm_page = reinterpret_cast<int32_t *>(sm_p + kSimtRows * (kN + 4));  // [kN]
   pdl_prologue();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t total = p.prefix[p.seq_count];
-  const int n = shares(p, total), share = blockIdx.x;
-  if (share >= n) return;
-  int64_t at = share_begin(total, n, share);
-  const int64_t end = share_begin(total, n, share + 1);
-  Place w = find_place(p, at);
+  const int share = blockIdx.x;
+  Place w;
+  int64_t left = find_share(p, share, &w);
+  if (left > 0 && w.off >= w.steps) next_tile(p, w);
   const int io = elem_bytes(p.io_code);
-  while (at < end) {
-    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + (end - at)));
+  while (left > 0) {
+    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
     const Piece x = piece_of(p, w, stop, share);
-    const float mul = score_mul(p, x.head), am = score_abs(mul);
+    const float mul = nonzero(score_mul(p, x.head)), am = fabsf(mul);
     __syncthreads();  // the previous piece is done with shared memory
     for (int i = tid; i < kSimtRows * dp; i += kSimtThreads) {
       const int row = i / dp, d = i - row * dp;
@@ -1476,7 +1697,7 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
         const int32_t r = x.row0 + row, token = r / p.group, h = x.head * p.group + (r - token * p.group);
         y = load_f32(p.query + (x.q.first + token) * p.q_pitch + (static_cast<int64_t>(h) * p.dim + d) * io, p.io_code);
       }
-      sm_q[row * pitch + d] = mul < 0.f ? -y : mul == 0.f ? 0.f : y;
+      sm_q[row * pitch + d] = mul < 0.f ? -y : y;
     }
     float acc[4][kPer], m[4], l[4];
     int32_t limit[4];
@@ -1556,7 +1777,7 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
         if (lane < kN) sm_p[row * (kN + 4) + lane] = wgt;
       }
       __syncthreads();  // V in place, weights in place
-#pragma unroll
+#pragma unroll 1
       for (int c0 = 0; c0 < kN; c0 += 4) {
         float4 wv[4];
 #pragma unroll
@@ -1600,8 +1821,8 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
       }
       if (x.slot >= 0 && lane == 0) reinterpret_cast<float2 *>(p.part_ml)[part] = make_float2(m[i], l[i]);
     }
-    at += stop - w.off;
-    if (at < end) next_tile(p, w);
+    left -= stop - w.off;
+    if (left > 0) next_tile(p, w);
   }
 }
 
@@ -1611,11 +1832,13 @@ constexpr int kMaxShares = 148;      // of the tensor-core kernel: one CTA per S
 constexpr int kMaxSimtShares = 296;  // of the f32 kernel
 constexpr int kMinShare = 2;         // steps; a shorter share costs more in its partial result than it saves
 constexpr int kMinSimtShare = 4;
+constexpr int kTileCost = 2;  // steps that loading a tile's queries and writing its result are worth
+constexpr int kSimtTileCost = 1;
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Split {
-  int32_t tile_rows, kv_tile, grid, slot_rows, min_share;
+  int32_t tile_rows, kv_tile, grid, slot_rows, min_share, tile_cost;
   size_t prefix_bytes, ml_bytes, o_bytes;
   size_t total() const { return prefix_bytes + ml_bytes + o_bytes; }
 };
@@ -1628,9 +1851,10 @@ Split split_of(bool tensor, int64_t seqs, int64_t rows, int64_t heads_q, int64_t
   s.tile_rows = tensor ? (dim > 128 ? kTile : 2 * kTile) : kSimtRows;
   s.kv_tile = tensor ? kTile : simt_tokens(static_cast<int>(dim > 512 ? 1024 : 64));
   s.min_share = tensor ? kMinShare : kMinSimtShare;
+  s.tile_cost = tensor ? kTileCost : kSimtTileCost;
   const int64_t most = tensor ? kMaxShares : (dim > 256 ? kMaxShares : kMaxSimtShares);
   const int64_t tiles = (seqs + rows * group / s.tile_rows) * heads_kv;
-  const int64_t per_tile = std::max<int64_t>(1, (max_len + s.kv_tile - 1) / s.kv_tile);
+  const int64_t per_tile = std::max<int64_t>(1, (max_len + s.kv_tile - 1) / s.kv_tile) + s.tile_cost;
   int64_t steps;
   if (__builtin_mul_overflow(tiles, per_tile, &steps)) steps = INT64_MAX / 2;
   s.grid = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(most, (steps + s.min_share - 1) / s.min_share)));
@@ -1683,22 +1907,61 @@ EncodeTiled encode_tiled() {
   return reinterpret_cast<EncodeTiled>(f);
 }
 
-// Pages as a 4-d tensor (dim, head and token in the order of their strides, page) loaded in boxes
-// of 64 dims x `box` tokens of one head of one page, swizzled as the operands want them.
-bool make_map(CUtensorMap *map, const ChunkParams &p, const PageView &v, bool bf16) {
+// Pages as a tensor that is loaded in boxes of `box` tokens of one head of one page, swizzled as the
+// operands want them.  Whole boxes: (64 dims, 8 tokens, panels, groups of 8 tokens, pages), with the
+// head folded into the panels (heads next to each other) or into the groups (heads behind each
+// other's tokens), so that all panels come with one box.  Otherwise (dim, head and token in the
+// order of their strides, page), one panel to a box; dims behind head_dim come as zeros.
+bool make_map(CUtensorMap *map, const ChunkParams &p, const PageView &v, bool bf16, int unit_panels) {
   const EncodeTiled encode = encode_tiled();
   if (encode == nullptr) return false;
-  const bool head_inner = p.k.head < p.k.tok;
+  const CUtensorMapDataType type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint64_t heads = static_cast<cuuint64_t>(p.heads_kv), toks = static_cast<cuuint64_t>(p.block_size);
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.dim), head_inner ? heads : toks, head_inner ? toks : heads,
-                              static_cast<cuuint64_t>(p.num_blocks)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(head_inner ? v.head : v.tok), static_cast<cuuint64_t>(head_inner ? v.tok : v.head),
+  const cuuint64_t pages = static_cast<cuuint64_t>(p.num_blocks);
+  if (p.whole_boxes) {
+    const cuuint64_t dims[5] = {64, 8, (heads - 1) * p.head_panels + p.dim / 64, (heads - 1) * p.head_groups + toks / 8, pages};
+    const cuuint64_t strides[4] = {static_cast<cuuint64_t>(v.tok), 128, static_cast<cuuint64_t>(v.tok) * 8, static_cast<cuuint64_t>(v.blk)};
+    const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(unit_panels), static_cast<cuuint32_t>(p.box / 8), 1};
+    const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+    return encode(map, type, 5, v.base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.dim), p.head_inner ? heads : toks, p.head_inner ? toks : heads, pages};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.head_inner ? v.head : v.tok), static_cast<cuuint64_t>(p.head_inner ? v.tok : v.head),
                                  static_cast<cuuint64_t>(v.blk)};
   const cuuint32_t rows = static_cast<cuuint32_t>(p.box);
-  const cuuint32_t box[4] = {64, head_inner ? 1 : rows, head_inner ? rows : 1, 1};
+  const cuuint32_t box[4] = {64, p.head_inner ? 1 : rows, p.head_inner ? rows : 1, 1};
   const cuuint32_t step[4] = {1, 1, 1, 1};
-  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, v.base, dims, strides, box, step,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return encode(map, type, 4, v.base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a head adds to the coordinates of whole boxes; false when K or V does not fold that way.
+bool fold_heads(ChunkParams *p) {
+  if (p->dim % 64 != 0) return false;
+  p->head_panels = p->head_groups = 0;
+  if (p->heads_kv == 1) return true;
+  const PageView &k = p->k, &v = p->v;
+  if (p->head_inner) {  // heads are panels further on
+    if (k.head != v.head || k.head % 128 != 0) return false;
+    p->head_panels = static_cast<int32_t>(k.head / 128);
+    return k.head / 128 * (p->heads_kv - 1) < INT32_MAX / 2;
+  }
+  if (k.head % (8 * k.tok) != 0 || v.head % (8 * v.tok) != 0 || k.head / k.tok != v.head / v.tok) return false;
+  p->head_groups = static_cast<int32_t>(k.head / (8 * k.tok));
+  return k.head / (8 * k.tok) * (p->heads_kv - 1) < INT32_MAX / 2;
+}
+
+// Query rows as a 3-d tensor (dim, head, token) loaded as the 128 rows of a stream.
+bool make_query_map(CUtensorMap *map, const ChunkParams &p, bool bf16) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.dim), static_cast<cuuint64_t>(p.heads_kv) * p.group, static_cast<cuuint64_t>(p.rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.dim) * 2, static_cast<cuuint64_t>(p.q_pitch)};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(kTile / p.group)};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<char *>(p.query), dims, strides,
+                box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1709,20 +1972,20 @@ bool tma_strides(const PageView &v) {
 }
 
 template <typename T, int kDp, bool kTma>
-void launch_tensor(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t st) {
+void launch_tensor(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, const CUtensorMap &q, cudaStream_t st) {
   const size_t smem = chunk_smem_bytes<kDp>();
   // (the attribute is per device and cheap to set, so it is set on every launch)
   cudaFuncSetAttribute(kvx_chunk_attention_kernel<T, kDp, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  launch_pdl(kvx_chunk_attention_kernel<T, kDp, kTma>, dim3(static_cast<unsigned>(p.grid)), kThreads, smem, st, p, k, v);
+  launch_pdl(kvx_chunk_attention_kernel<T, kDp, kTma>, dim3(static_cast<unsigned>(p.grid)), kThreads, smem, st, p, k, v, q);
 }
 template <typename T, bool kTma>
-void launch_tensor_dim(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t st) {
+void launch_tensor_dim(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, const CUtensorMap &q, cudaStream_t st) {
   if (p.dim <= 64)
-    launch_tensor<T, 64, kTma>(p, k, v, st);
+    launch_tensor<T, 64, kTma>(p, k, v, q, st);
   else if (p.dim <= 128)
-    launch_tensor<T, 128, kTma>(p, k, v, st);
+    launch_tensor<T, 128, kTma>(p, k, v, q, st);
   else
-    launch_tensor<T, 256, kTma>(p, k, v, st);
+    launch_tensor<T, 256, kTma>(p, k, v, q, st);
 }
 template <int kDb>
 void launch_simt(const ChunkParams &p, cudaStream_t st) {
@@ -1816,6 +2079,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   p.max_seq_len = static_cast<int32_t>(attn->max_seq_len);
   p.num_blocks = static_cast<int32_t>(cache->num_blocks);
   p.block_size = static_cast<int32_t>(cache->block_size);
+  p.bs_shift = (p.block_size & (p.block_size - 1)) == 0 ? __builtin_ctz(cache->block_size) : -1;
   p.heads_kv = static_cast<int32_t>(H);
   p.group = static_cast<int32_t>(group);
   p.dim = static_cast<int32_t>(D);
@@ -1829,6 +2093,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   p.min_share = sp.min_share;
   p.tile_rows = sp.tile_rows;
   p.kv_tile = sp.kv_tile;
+  p.tile_cost = sp.tile_cost;
   p.pair = tensor && D <= 128 ? 1 : 0;
   p.q_vec = D % 8 == 0 && p.q_pitch % 16 == 0 && p.o_pitch % 16 == 0 && aligned16(p.query) && aligned16(p.out) ? 1 : 0;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
@@ -1842,8 +2107,20 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
       if (p.v.head <= 0 || p.v.head % 16 != 0) p.v.head = p.v.tok;
     }
     CUtensorMap kmap = {}, vmap = {};
+    const int unit_panels = D <= 64 ? 1 : 2;
+    const bool bf16 = io == KVX_DTYPE_BF16;
+    p.head_inner = p.k.head < p.k.tok ? 1 : 0;
     bool tma = elem == 2 && p.box >= 8 && tma_strides(p.k) && tma_strides(p.v) && (p.k.head < p.k.tok) == (p.v.head < p.v.tok);
-    tma = tma && make_map(&kmap, p, p.k, io == KVX_DTYPE_BF16) && make_map(&vmap, p, p.v, io == KVX_DTYPE_BF16);
+    p.whole_boxes = tma && fold_heads(&p) ? 1 : 0;
+    if (p.whole_boxes && !(make_map(&kmap, p, p.k, bf16, unit_panels) && make_map(&vmap, p, p.v, bf16, unit_panels))) p.whole_boxes = 0;
+    if (tma && !p.whole_boxes) tma = make_map(&kmap, p, p.k, bf16, unit_panels) && make_map(&vmap, p, p.v, bf16, unit_panels);
+    p.group_stride = p.whole_boxes ? unit_panels * 1024 : 1024;
+    p.panel_stride = p.whole_boxes ? 1024 : kPanelBytes;
+    CUtensorMap qmap = {};
+    p.q_tma = p.q_vec && (p.group & (p.group - 1)) == 0 && p.group <= kTile && p.q_pitch < (int64_t{1} << 40) &&
+                      make_query_map(&qmap, p, io == KVX_DTYPE_BF16)
+                  ? 1
+                  : 0;
     const int64_t piece = 8 * elem;  // bytes one lane copies at a time where TMA is not used
     auto rows_ok = [&](const PageView &v) {
       return v.pack == 1 && v.dhi == elem && reinterpret_cast<uintptr_t>(v.base) % piece == 0 && v.blk % piece == 0 && v.tok % piece == 0 &&
@@ -1852,14 +2129,14 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
     p.kv_vec = D % 8 == 0 && rows_ok(p.k) && rows_ok(p.v) ? 1 : 0;
     if (io == KVX_DTYPE_BF16) {
       if (tma)
-        launch_tensor_dim<Bf16, true>(p, kmap, vmap, cs);
+        launch_tensor_dim<Bf16, true>(p, kmap, vmap, qmap, cs);
       else
-        launch_tensor_dim<Bf16, false>(p, kmap, vmap, cs);
+        launch_tensor_dim<Bf16, false>(p, kmap, vmap, qmap, cs);
     } else {
       if (tma)
-        launch_tensor_dim<Fp16, true>(p, kmap, vmap, cs);
+        launch_tensor_dim<Fp16, true>(p, kmap, vmap, qmap, cs);
       else
-        launch_tensor_dim<Fp16, false>(p, kmap, vmap, cs);
+        launch_tensor_dim<Fp16, false>(p, kmap, vmap, qmap, cs);
     }
   } else if (D <= 64) {
     launch_simt<64>(p, cs);

@@ -1007,7 +1007,13 @@ __device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, ui
   }
 }
 
-// ---- products -----------------------------------------------------------------------------
+// ---- products -----
+//
+// A tcgen05.commit that follows another one waits in the issuing warp until the products ahead of the
+// first have ended (about 800 clocks here), so there is one commit per group of products: scores
+// announce themselves and with them every product issued earlier.  What else waits for the products
+// -- the rings, the query tile -- is told by the softmax warps.
+//------------------------------------------------------------------------
 
 template <typename T, int kDp>
 struct Products {
@@ -1033,11 +1039,7 @@ struct Products {
       if (!warp_wait(smem_addr(&m->kv_full[ring.slot()]), ring.phase())) return false;
     return true;
   }
-  __device__ __forceinline__ void release(Ring<kDp> &ring) {
-#pragma unroll
-    for (int u = 0; u < S::kUnits; ++u, ++ring.entry) tc_commit(elected, smem_addr(&m->kv_empty[ring.slot()]));
-  }
-  __device__ __forceinline__ void scores(uint32_t s, bool free_q) {
+  __device__ __forceinline__ void scores(uint32_t s) {
     tc_fence_after();
     const uint32_t buf = S::kScoreBufs == 2 ? (tiles++ & 1) : s;
     const uint32_t d = tmem + buf * kTile;
@@ -1054,11 +1056,10 @@ struct Products {
       }
     }
     tc_commit(elected, smem_addr(&m->s_full[0]) + 8 * buf);
-    if (free_q) tc_commit(elected, smem_addr(&m->q_empty[0]) + 8 * s);
   }
   // The product over the first three quarters of the tokens runs while the last weights are still
   // being made.
-  __device__ __forceinline__ bool output(uint32_t s, bool first) {
+  __device__ __forceinline__ bool output(uint32_t s, bool first, bool last) {
     const uint32_t buf = S::kScoreBufs == 2 ? (weights & 1) : s;
     const uint32_t ph = S::kScoreBufs == 2 ? (weights >> 1 & 1) : (p_phase >> s & 1);
     const uint32_t a = tmem + buf * kTile, d = tmem + 256 + s * kDp;
@@ -1081,7 +1082,8 @@ struct Products {
 #pragma unroll
       for (int kk = 6; kk < 8; ++kk) mma_ts(elected, d + u * 128, a + kk * 8, vd + kk * step, kOutput, 1);
     }
-    tc_commit(elected, smem_addr(&m->pv_done[0]) + 8 * s);
+    // two streams: until the last tile, the stream's next scores tell that this product has ended
+    if (S::kScoreBufs == 2 || last) tc_commit(elected, smem_addr(&m->pv_done[0]) + 8 * s);
     p_phase ^= 1u << s;
     ++weights;
     return true;
@@ -1102,8 +1104,6 @@ struct Products {
       if (!warp_wait(smem_addr(&m->q_full[s]), q_phase >> s & 1)) return false;
       q_phase ^= 1u << s;
     }
-    // the query tile of stream 1 is the join's buffer first
-    const bool joins = __any_sync(0xFFFFFFFFu, joins_streams(x)) != 0;
     const bool narrow = S::kStreams == 2 && __any_sync(0xFFFFFFFFu, x.narrow) != 0;
     const int most = max(n0, n1);
     if (most == 0) return true;
@@ -1112,37 +1112,33 @@ struct Products {
       if (S::kStreams == 1) {  // scores of the next tile ahead of the output product of this one
         if (i < most) {
           if (!acquire(k_ring)) return false;
-          scores(0, p.q_tma && i + 1 == most);
-          release(k_ring);
+          scores(0);
+          k_ring.entry += S::kUnits;
         }
         if (i > 0) {
-          if (!acquire(v_ring) || !output(0, i == 1)) return false;
-          release(v_ring);
+          if (!acquire(v_ring) || !output(0, i == 1, i == most)) return false;
+          v_ring.entry += S::kUnits;
         }
         continue;
       }
       bool has_k = false, has_v = false;
-#pragma unroll 1
+#pragma unroll
       for (uint32_t s = 0; s < 2; ++s) {
         const int n = s == 0 ? n0 : n1;
-        const bool done = narrow || s == 1;  // the tile's last reader
         if (i > 0 && i <= n) {
           if (!has_v && !acquire(v_ring)) return false;
           has_v = true;
-          if (!output(s, i == 1)) return false;
-        }
-        if (has_v && done) {
-          release(v_ring);
-          has_v = false;
+          if (!output(s, i == 1, i == n)) return false;
         }
         if (i < n) {
           if (!has_k && !acquire(k_ring)) return false;
           has_k = true;
-          scores(s, p.q_tma && i + 1 == n && !(s == 1 && joins));
+          scores(s);
         }
-        if (has_k && done) {
-          release(k_ring);
-          has_k = false;
+        if (narrow || s == 1) {  // the tiles' last reader
+          v_ring.entry += has_v;
+          k_ring.entry += has_k;
+          has_k = has_v = false;
         }
       }
     }
@@ -1157,43 +1153,20 @@ struct Products {
 // sums in tensor memory are rescaled on a few tiles instead of on every one.
 constexpr float kLazy = 8.f;
 
-#ifndef KVX_CHUNK_POLY
-#define KVX_CHUNK_POLY 2  // pairs of 8 whose exponentials are made by exp2_pair
-#endif
-
-// 2^z on the f32 pipes, for a pair: the exponent unit alone (16 results per clock and SM) would be
-// what bounds the kernel.  z = n + f with n the nearest integer (its bits appear in the low end of
-// z + kRound); 2^f by a polynomial of degree 4 on [-1/2, 1/2], fitted for the least relative error
-// (2^-18.5, well below the 2^-9 or 2^-12 that rounding a weight costs); times the float whose
-// exponent field is n + 127.  z is held at -127 or above, where that field, and the result, is zero;
-// a NaN stays one.
-__device__ __forceinline__ float2 exp2_pair(float2 z) {
-  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23, and the exponent bias
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.x) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.y) : "f"(-127.f));
-  const float2 r = __fadd2_rn(z, make_float2(kRound, kRound));
-  const float2 n = __fadd2_rn(r, make_float2(-kRound, -kRound));
-  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), z);
-  float2 y = __ffma2_rn(make_float2(0.00957053154706955f, 0.00957053154706955f), f, make_float2(0.05591866374015808f, 0.05591866374015808f));
-  y = __ffma2_rn(y, f, make_float2(0.24024735391139984f, 0.24024735391139984f));
-  y = __ffma2_rn(y, f, make_float2(0.6931216716766357f, 0.6931216716766357f));
-  y = __ffma2_rn(y, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-  return __fmul2_rn(y, make_float2(__uint_as_float(__float_as_uint(r.x) << 23), __uint_as_float(__float_as_uint(r.y) << 23)));
-}
-
-// Weights of 16 scores of one row: exponentials, their sum, and the rounded pairs to tensor memory.
+// Weights of 32 scores of one row: exponentials, their sum, and the rounded pairs to tensor memory.
+// (Making a quarter of the exponentials by a polynomial on the f32 pipes was slower: the softmax warps
+// are bound by the latency of their own instructions, not by the exponential unit.)
 template <typename T>
 __device__ __forceinline__ void weigh(const float *sc, float2 mul2, float2 sub2, float2 &sum2, uint32_t to) {
-  uint32_t w[8];
+  uint32_t w[16];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < 16; ++k) {
     const float2 z = __ffma2_rn(make_float2(sc[2 * k], sc[2 * k + 1]), mul2, sub2);
-    const bool poly = (k + 1) * KVX_CHUNK_POLY / 8 != k * KVX_CHUNK_POLY / 8;  // spread evenly
-    const float2 y = poly ? exp2_pair(z) : make_float2(fast_exp2(z.x), fast_exp2(z.y));
+    const float2 y = make_float2(fast_exp2(z.x), fast_exp2(z.y));
     sum2 = __fadd2_rn(sum2, y);
     w[k] = T::pack2(y.x, y.y);
   }
-  tc_st8(to, w);
+  tc_st16(to, w);
 }
 
 // Whether the page of this lane's four tokens of the tile at `first` exists; page sizes that are not a
@@ -1266,8 +1239,17 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
   const int s = threadIdx.x >> 7;                 // stream
   const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
   const uint32_t lanes = static_cast<uint32_t>((tid >> 5) * 32) << 16;  // this warp's lanes of tensor memory
-  uint32_t tiles = 0;  // score tiles of this stream so far
+  uint32_t tiles = 0;   // score tiles of this stream so far
+  uint32_t pieces = 0;  // pieces of this stream that had any
   uint32_t joins = 0;
+  uint32_t entries = 0;  // tiles of both rings before this piece
+  // The ring entries of a K or V tile (the `q`-th of the piece) may be filled again.
+  auto release = [&](int which, int q) {
+    if (tid != 0) return;
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u)
+      mbar_arrive(smem_addr(&m->kv_empty[0]) + 8 * (which * S::kRing + (((entries + q) * S::kUnits + u) & (S::kRing - 1))));
+  };
 #pragma unroll 1
   for (uint32_t item = 0;; ++item) {
     const uint32_t slot = item % kItems;
@@ -1276,12 +1258,24 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_addr(&m->item_empty[slot]));
     if (x.rows == 0) return;
-    int b, e;
+    int b, e, other = 0;  // tiles of this stream, number of the other stream's
     stream_range<S::kStreams>(p, x, s, &b, &e);
+    if (S::kStreams == 2) {
+      int ob, oe;
+      stream_range<S::kStreams>(p, x, s ^ 1, &ob, &oe);
+      other = oe - ob;
+    }
     const bool narrow = S::kStreams == 2 && x.narrow;
+    const int count = narrow ? e - b + other : max(e - b, other);  // tiles of the piece, each of K and of V
+    // this stream is the last reader of its tile i (stream 1 comes after stream 0)
+    auto last_reader = [&](int i) { return narrow || s == 1 || i >= other; };
+    auto place = [&](int i) { return narrow ? 2 * i + s : i; };
     const int32_t row_at = x.row0 + (narrow ? 0 : s * kTile);   // first group row of this stream
     const int32_t rows = min(kTile, x.rows - (narrow ? 0 : s * kTile));
-    if (rows <= 0) continue;
+    if (rows <= 0) {
+      entries += count;
+      continue;
+    }
     const float mul = nonzero(score_mul(p, x.head));
     const float am = fabsf(mul), sign = mul > 0.f ? 1.f : -1.f;
 
@@ -1337,6 +1331,11 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
       const bool gaps = __all_sync(0xFFFFFFFFu, page_ok) == 0;
       if (!warp_wait(smem_addr(&m->s_full[0]) + 8 * buf, ph)) return;
       tc_fence_after();
+      // these scores have read their K tile, and (two streams) the product ahead of them its V tile
+      const int i = j - b;
+      if (last_reader(i)) release(0, place(i));
+      if (S::kStreams == 2 && i > 0 && last_reader(i - 1)) release(1, place(i - 1));
+      if (j == e - 1 && p.q_tma && tid == 0 && !(s == 1 && joins_streams(x))) mbar_arrive(smem_addr(&m->q_empty[0]) + 8 * s);
       if (!plain) correct_scores(p, x, s_at, j * kTile, valid, gaps, sign);
       float top = -INFINITY;
 #pragma unroll 1
@@ -1362,8 +1361,9 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
         if (raise) mx = top;
         if (j > b) {
           l *= c;
-          // the sums of the tiles so far must be complete before they are rescaled
-          if (!warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (tiles - 1) & 1)) return;
+          // the sums of the tiles so far must be complete before they are rescaled (two streams: they
+          // are, these scores were announced behind them)
+          if (S::kStreams == 1 && !warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
           tc_fence_after();
 #pragma unroll 1
           for (int k = 0; k < kDp; k += 16) {
@@ -1381,29 +1381,33 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
       const float2 mul2 = make_float2(am, am), sub2 = make_float2(sub, sub);
       float2 sum2 = make_float2(0.f, 0.f);
       {
-        // 16 columns at a time, the next 16 on their way; the weights of columns c, c + 1 go to column
+        // 32 columns at a time, the next 32 on their way; the weights of columns c, c + 1 go to column
         // c / 2, which has been read by then.
-        float c0[16], c1[16];
-        tc_ld16(c0, s_at);
+        float c0[32], c1[32];
+        tc_ld32(c0, s_at);
 #pragma unroll 1
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2; ++k) {
           tc_wait_ld();
-          tc_ld16(c1, s_at + 32 * k + 16);
-          if (k == 3) {
+          tc_ld32(c1, s_at + 64 * k + 32);
+          weigh<T>(c0, mul2, sub2, sum2, s_at + 32 * k);
+          tc_wait_ld();
+          if (k == 0) {
+            tc_ld32(c0, s_at + 64);
+          } else {
             // Three quarters are made.  One stream: the scores of this tile were issued ahead of the
             // previous output product, so they do not tell that it has ended.  Weights are handed over
             // only after it has -- its barrier is then never more than one phase away from the
             // parity that is waited for.
-            if (S::kScoreBufs == 2 && j > b && !warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (tiles - 1) & 1)) return;
+            if (S::kStreams == 1 && j > b) {
+              if (!warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
+              release(1, i - 1);
+            }
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&m->p_part[0]) + 8 * buf);
           }
-          weigh<T>(c0, mul2, sub2, sum2, s_at + 16 * k);
-          tc_wait_ld();
-          if (k < 3) tc_ld16(c0, s_at + 32 * k + 32);
-          weigh<T>(c1, mul2, sub2, sum2, s_at + 16 * k + 8);
+          weigh<T>(c1, mul2, sub2, sum2, s_at + 32 * k + 16);
         }
       }
       l += sum2.x + sum2.y;
@@ -1415,9 +1419,12 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
 
     // ---- the piece's result ----
     if (e > b) {
-      if (!warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (tiles - 1) & 1)) return;
+      if (!warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (S::kStreams == 1 ? tiles - 1 : pieces) & 1)) return;
       tc_fence_after();
+      ++pieces;
+      if (last_reader(e - b - 1)) release(1, place(e - b - 1));
     }
+    entries += count;
     const float vmul = p.vs.base != nullptr ? p.vs.base[x.head * p.vs.stride] : 1.f;
     const bool join = S::kStreams == 2 && joins_streams(x);
     // Stream 1 hands its sums to stream 0 through its query tile, [kDp / 2][128] at a time.
@@ -1577,12 +1584,15 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
   }
 }
 
-// The kernel's code size is part of its speed: warps of five roles run different code at the same
-// time, and straight-line code that is not in the instruction caches runs at about 8 clocks an
-// instruction.  Loops over columns are therefore kept as loops of 32 to 64 columns, every role has
-// one call site per large routine, and branches on the stream number are avoided (the compiler
-// would clone the loop per stream).  266 KB of code against 60 KB: 1.82 against 1.3 ms for 16 prompts
-// of 512 to 4096 tokens.
+// Every role's instruction count is part of the kernel's speed: a single warp gets through about one
+// instruction in eight clocks here, so loops over columns are kept as loops of 32 to 64 columns that
+// fit the registers, and what is done per tile by the loading and the issuing warps is kept small.
+// Measured on 16 prompts of 512 to 4096 tokens and on 4 x 512 tokens over 32k contexts (us):
+//   first version, one thread issuing everything, boxes issued by their lanes     2410   1310
+//   queries by TMA, column loops, waits that do not read the timer first          1290   1110 - 1250
+//   + whole boxes, two loading warps, converged issue, one commit per product     1200   1110 - 1220
+// Two warps per 32 rows (half the columns each, 640 threads) ran at 1470 and 1340; keeping all 128
+// scores of a row in registers at 1440 and 1320; strict turns between the streams changed nothing.
 template <typename T, int kDp, bool kTma>
 __global__ void __launch_bounds__(kThreads, 1)
     kvx_chunk_attention_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,

@@ -66,7 +66,7 @@ struct ChunkParams {
   int32_t head_inner;          // else: heads are closer together than tokens
   int32_t q_tma;               // 1: query tiles are loaded by TMA
   int32_t q_vec;               // 1: query rows can be read, out rows written in 16-byte pieces
-  int32_t kv_vec;              // 1: page rows can be read in pieces of 8 elements
+  int32_t kv_vec;              // 1: page rows can be read in 16-byte pieces
 };
 
 __device__ int g_chunk_error;  // set to 1 when a bounded wait gave up
@@ -616,12 +616,13 @@ struct Fp16 {
 
 // ------------------------------------------------------------------ tensor-core kernel --
 //
-// Roles of a CTA (one per SM, 384 threads):
+// Roles of a CTA (one per SM, 384 threads, 512 where loading takes more than TMA):
 //   warps 0-3, 4-7   softmax of stream 0 and of stream 1: a thread owns one of the 128 rows
 //   warp 8           issues every tcgen05.mma
 //   warp 9           walks the schedule, publishes pieces, loads Q and K tiles (TMA)
 //   warp 10          loads V tiles
-//   (warps 9 to 11   copy K and V tiles where pages cannot be read by TMA)
+//   (e4m3: warp 9 loads K and V bytes, warps 10 to 15 convert them; pages that TMA cannot read:
+//   warps 9 to 15 copy them)
 // Two streams of 128 rows keep the tensor pipe and the exponentials busy in turn: while one
 // stream's scores are turned into weights the other stream's products run.  A tile with at most
 // 128 rows gives both streams the same rows and every K/V tile to one of them; the two halves are
@@ -633,8 +634,11 @@ struct Fp16 {
 // the order of their issue, which is what lets the scores of the next tile overwrite the weights
 // the previous product read.
 
-constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8;
+// How K and V get into shared memory.
+enum Loads { kTmaLoads, kRawLoads, kCopyLoads };  // TMA; e4m3 bytes by TMA, converted; copied by warps
+constexpr int kCopyWarps = 7, kConvertWarps = 6;
+constexpr int threads_of(Loads loads) { return loads == kTmaLoads ? 384 : 512; }
 constexpr int kTile = 128;          // rows of a stream, tokens of a K/V tile
 constexpr int kPanelBytes = 16384;  // 128 rows x 128 bytes
 constexpr int kItems = 2;           // pieces published ahead
@@ -650,7 +654,9 @@ struct Shape {
   static constexpr int kRing = kDp == 64 ? 4 : 2;          // entries of the K ring and of the V ring (powers of two)
   static constexpr int kQBytes = kPanels * kPanelBytes;    // per stream
   static constexpr int kRingAt = kStreams * kQBytes;
-  static constexpr int kMiscAt = kRingAt + 2 * kRing * kUnitBytes;
+  static constexpr int kRawBytes = kTile * kUnitPanels * 64;  // an entry's e4m3 bytes
+  static constexpr int kRawAt = kRingAt + 2 * kRing * kUnitBytes;
+  static constexpr int kMiscAt = kRawAt + 2 * kRawBytes;
 };
 
 struct Misc {
@@ -658,6 +664,7 @@ struct Misc {
   uint64_t kv_full[8], kv_empty[8];
   uint64_t q_full[2], q_empty[2], s_full[2], p_part[2], p_full[2], pv_done[2];
   uint64_t join_full, join_empty;
+  uint64_t raw_full[2], raw_empty[2];
   uint64_t tail, drain;
   Piece items[kItems];
   float join_m[kTile], join_l[kTile];
@@ -746,6 +753,53 @@ struct Ring {
 
 // ---- loads ------------------------------------------------------------------------------
 
+// The pieces of this CTA's share, one after the other; behind the last a piece without rows.  All lanes
+// of a warp call it together.
+struct Schedule {
+  Place w;
+  int64_t left;
+  __device__ __forceinline__ explicit Schedule(const ChunkParams &p) {
+    left = find_share(p, blockIdx.x, &w);
+    if (left > 0 && w.off >= w.steps) next_tile(p, w);
+  }
+  __device__ __forceinline__ Piece next(const ChunkParams &p) {
+    Piece x;
+    x.rows = 0;
+    if (left > 0) {
+      const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
+      x = piece_of(p, w, stop, blockIdx.x);
+      left -= stop - w.off;
+      if (left > 0) next_tile(p, w);
+    }
+    return x;
+  }
+};
+
+// Hands piece `item` to the other warps, and its queries to TMA.
+template <int kDp>
+__device__ __forceinline__ bool publish(const ChunkParams &p, const CUtensorMap *qmap, const Piece &x, uint32_t item, uint32_t base, Misc *m,
+                                        uint32_t elected, uint32_t *queries) {
+  const uint32_t slot = item % kItems;
+  if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1)) return false;
+  bool ok = true;
+  if (elected) {
+    m->items[slot] = x;
+    mbar_arrive(smem_addr(&m->item_full[slot]));
+    if (p.q_tma && x.rows > 0) ok = load_queries<kDp>(p, qmap, x, base, m, queries);
+  }
+  return __all_sync(0xFFFFFFFFu, ok) != 0;
+}
+// Takes piece `item`.
+__device__ __forceinline__ bool receive(Misc *m, uint32_t item, uint32_t elected, Piece *x) {
+  const uint32_t slot = item % kItems;
+  if (!warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1)) return false;
+  *x = m->items[slot];
+  __syncwarp();
+  if (elected) mbar_arrive(smem_addr(&m->item_empty[slot]));
+  __syncwarp();
+  return true;
+}
+
 // Two warps load by TMA: the first walks the schedule, publishes the pieces, loads the queries and the
 // K tiles, the second loads the V tiles.  What a single warp does per box and per tile is on the
 // kernel's critical path (one instruction every ten clocks or so), so a box carries all panels of
@@ -830,47 +884,18 @@ __device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, con
     return true;
   };
   bool ok = true;
-  Place w;
-  int64_t left = 0;
-  if (!mine_v) {
-    left = find_share(p, blockIdx.x, &w);
-    if (left > 0 && w.off >= w.steps) next_tile(p, w);
-  }
+  Schedule schedule(p);
 #pragma unroll 1
-  for (uint32_t item = 0;; ++item) {
-    const uint32_t slot = item % kItems;
+  for (uint32_t item = 0; ok; ++item) {
     Piece x;
     if (mine_v) {
-      ok = warp_wait(smem_addr(&m->item_full[slot]), (item / kItems) & 1);
-      if (!ok) break;
-      x = m->items[slot];
-      __syncwarp();
-      if (elected) mbar_arrive(smem_addr(&m->item_empty[slot]));
+      ok = receive(m, item, elected, &x);
     } else {
-      // one piece more than there is, without rows: the end
-      if (item >= kItems) ok = warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1);
-      if (!ok) break;
-      x.rows = 0;
-      if (left > 0) {
-        const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
-        x = piece_of(p, w, stop, blockIdx.x);
-        left -= stop - w.off;
-        if (left > 0) next_tile(p, w);
-      }
-      if (elected) {
-        m->items[slot] = x;
-        mbar_arrive(smem_addr(&m->item_full[slot]));
-      }
-      __syncwarp();
+      x = schedule.next(p);
+      ok = publish<kDp>(p, qmap, x, item, base, m, elected, queries);
     }
-    if (__all_sync(0xFFFFFFFFu, x.rows == 0)) break;
-    if (!mine_v && p.q_tma) {
-      if (elected) ok = load_queries<kDp>(p, qmap, x, base, m, queries);
-      ok = __all_sync(0xFFFFFFFFu, ok) != 0;
-      if (!ok) break;
-    }
+    if (!ok || __all_sync(0xFFFFFFFFu, x.rows == 0)) break;
     ok = load_piece(x);
-    if (!ok) break;
   }
   // Nothing may be in flight towards this CTA's shared memory when it ends.  Normally: every
   // entry's release has arrived.  After giving up: the loads themselves, as far as they come.
@@ -885,117 +910,157 @@ __device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, con
   }
 }
 
-// Pages that TMA cannot read (e4m3, HND_PACKED, odd page sizes, odd strides): three warps copy rows
-// into the same swizzled tiles, converting on the way.  Warp 9 walks the schedule here, too.
+// 16 bytes, or zeros; no branch, so that several loads of a lane are in flight together.
+__device__ __forceinline__ uint4 load16_if(bool there, const char *from) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+  asm volatile(
+      "{ .reg .pred q;\n\t"
+      "setp.ne.u32 q, %5, 0;\n\t"
+      "@q ld.global.v4.u32 {%0,%1,%2,%3}, [%4]; }"
+      : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
+      : "l"(from), "r"(static_cast<uint32_t>(there)));
+  return r;
+}
+
+// Eight elements of one token's head from `d` on, element by element; behind head_dim zeros.  e4m3 in
+// the first two words, 16-bit elements in all four.
+__device__ __noinline__ uint4 gather_elements(const PageView &view, const char *page, int32_t o, int32_t head, int32_t d, int32_t dim, int elem) {
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int c = 0; c < 8 && d + c < dim; ++c) {
+    const char *src = page + head_offset(view, o, head, d + c);
+    if (elem == 2)
+      w[c >> 1] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(src)) << ((c & 1) * 16);
+    else
+      w[c >> 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint8_t *>(src)) << ((c & 3) * 8);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Pages that TMA cannot read as operands (e4m3, HND_PACKED, odd page sizes, odd strides): seven warps
+// copy rows into the same swizzled tiles, converting on the way.  A warp's load instruction covers
+// whole rows in 16-byte pieces; pages are looked up a tile ahead, and the loads of an entry are in
+// flight while the one before it is converted.  Each warp walks the schedule for itself, the first
+// one publishes the pieces.
 template <typename T, int kDp>
 __device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, uint32_t base, Misc *m) {
   using S = Shape<kDp>;
-  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - (kMmaWarp + 1), tid = threadIdx.x - (kMmaWarp + 1) * 32;
+  constexpr int kPieces = S::kUnitPanels * 4;  // 16-byte pieces of a row of e4m3 (twice as many of 16-bit elements)
+  constexpr int kSteps = (4 * kPieces + kCopyWarps - 1) / kCopyWarps;  // loads of a lane and entry (twice as many ..)
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - (kMmaWarp + 1);
   Ring<kDp> rings[2] = {Ring<kDp>(base, 0), Ring<kDp>(base, 1)};
-  uint32_t item = 0, queries[2] = {0, 0};
-  const int share = blockIdx.x;
-  Place w;
-  int64_t left = find_share(p, share, &w);
-  if (left > 0 && w.off >= w.steps) next_tile(p, w);
-  const int elem = elem_bytes(p.cache_code);
-  while (left > 0) {
-    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
-    const Piece x = piece_of(p, w, stop, share);
-    if (warp == 0) {
-      const uint32_t slot = item % kItems;
-      if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1)) return;
-      bool ok = true;
-      if (lane == 0) {
-        m->items[slot] = x;
-        mbar_arrive(smem_addr(&m->item_full[slot]));
-        if (p.q_tma) ok = load_queries<kDp>(p, qmap, x, base, m, queries);
+  uint32_t queries[2] = {0, 0};
+  const uint32_t elected = elect_lane();
+  Schedule schedule(p);
+  const bool wide = p.cache_code != KVX_DTYPE_F8_E4M3;  // 16-bit elements
+  const int elem = wide ? 2 : 1, pieces = wide ? 2 * kPieces : kPieces;
+  const int in_group = lane / pieces, piece = lane % pieces;
+  auto row_of = [&](int k) { return (warp + kCopyWarps * k) * (32 / pieces) + in_group; };  // of load k; 128 and more: none
+
+  int32_t page[kSteps], next_page[kSteps];  // e4m3: of the rows in the tile being fetched, and in the one after it
+  auto look_up = [&](const Piece &x, int tile, int row) {
+    const int32_t tok = tile * kTile + row;
+    return row < kTile && tok < x.q.len ? page_of(p, x.seq, tok) : -1;
+  };
+  // Entry n of a piece is (tile, K or V, unit): K and V of a tile, then the next tile's.
+  auto fetch = [&](const Piece &x, const TileOrder &order, int n, int first, uint4 *r) {
+    const int u = n % S::kUnits, kv = n / S::kUnits & 1, q = n / (2 * S::kUnits), tile = order.tile(q);
+    if (!wide && u == 0 && kv == 0) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        page[k] = q == 0 ? look_up(x, tile, row_of(k)) : next_page[k];
+        next_page[k] = q + 1 < order.count ? look_up(x, order.tile(q + 1), row_of(k)) : -1;
       }
-      if (!__all_sync(0xFFFFFFFFu, ok)) return;
     }
-    ++item;
-    const TileOrder order = tile_order<S::kStreams>(p, x);
-    // (a V tile is consumed after the K tile behind it has been asked for)
+    const PageView &view = kv ? p.v : p.k;
+    const int d = u * S::kUnitPanels * 64 + piece * (16 / elem);
+    const char *const in_head = view.base + x.head * view.head + d * elem;
+    if (p.kv_vec) {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int32_t pg = wide ? look_up(x, tile, row_of(first + k)) : page[k];
+        const int32_t tok = tile * kTile + row_of(first + k);
+        const int32_t o = p.bs_shift >= 0 ? tok & (p.block_size - 1) : tok % p.block_size;
+        r[k] = load16_if(pg >= 0 && d < p.dim, in_head + pg * view.blk + o * view.tok);
+      }
+      return;
+    }
 #pragma unroll 1
-    for (int q = 0; q < 2 * order.count; ++q) {
-      const bool is_v = (q & 1) != 0;
-      const int tile = order.tile(q >> 1);
-      const PageView &view = is_v ? p.v : p.k;
-      Ring<kDp> &ring = rings[is_v];
-#pragma unroll 1
-      for (int u = 0; u < S::kUnits; ++u, ++ring.entry) {
-        const uint32_t st = ring.slot();
-        if (ring.entry >= S::kRing && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase() ^ 1)) return;
-        const uint32_t dst = ring.addr();
-        constexpr int kChunks = S::kUnitPanels * 8;  // 16-byte pieces of a row in this unit
-        constexpr int kBatch = 4;
-        for (int i0 = tid; i0 < kTile * kChunks; i0 += 96 * kBatch) {
-          uint4 r[kBatch];
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            const int i = i0 + 96 * k;
-            r[k] = make_uint4(0, 0, 0, 0);
-            if (i >= kTile * kChunks) continue;
-            const int row = i / kChunks, d = u * S::kUnitPanels * 64 + (i % kChunks) * 8;
-            const int32_t tok = tile * kTile + row;
-            if (tok >= x.q.len || d >= p.dim) continue;
-            const int32_t page = page_of(p, x.seq, tok);
-            if (page < 0) continue;
-            const char *from = view.base + page * view.blk;
-            const int32_t o = tok % p.block_size;
-            if (p.kv_vec) {
-              const char *src = from + o * view.tok + x.head * view.head + static_cast<int64_t>(d) * elem;
-              if (elem == 2)
-                r[k] = *reinterpret_cast<const uint4 *>(src);
-              else
-                *reinterpret_cast<uint2 *>(&r[k]) = *reinterpret_cast<const uint2 *>(src);
-            } else {
-              uint16_t e[8];
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                e[c] = 0;
-                if (d + c < p.dim) {
-                  const char *src = from + head_offset(view, o, x.head, d + c);
-                  e[c] = elem == 2 ? *reinterpret_cast<const uint16_t *>(src) : *reinterpret_cast<const uint8_t *>(src);
-                }
-              }
-              if (elem == 2)
-                r[k] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-              else
-                r[k] = make_uint4(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24, 0, 0);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < kBatch; ++k) {
-            const int i = i0 + 96 * k;
-            if (i >= kTile * kChunks) continue;
-            uint4 y = r[k];
-            if (elem == 1) {
-              uint32_t h[4];
-              asm("{ .reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b; }"
-                  : "=r"(h[0]), "=r"(h[1]) : "r"(r[k].x));
-              asm("{ .reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b; }"
-                  : "=r"(h[2]), "=r"(h[3]) : "r"(r[k].y));
-              y = make_uint4(T::from_f16x2(h[0]), T::from_f16x2(h[1]), T::from_f16x2(h[2]), T::from_f16x2(h[3]));
-            }
-            const int row = i / kChunks, c = i % kChunks;
-            const uint32_t to = dst + (c >> 3) * p.panel_stride + (row >> 3) * p.group_stride + (row & 7) * 128 + (((c & 7) ^ (row & 7)) << 4);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
-          }
+    for (int k = 0; k < kSteps; ++k) {
+      const int row = row_of(first + k);
+      const int32_t pg = look_up(x, tile, row);
+      uint4 y = make_uint4(0, 0, 0, 0);
+      if (pg >= 0 && d < p.dim) {
+        const int32_t o = (tile * kTile + row) % p.block_size;
+        const char *from = view.base + pg * view.blk;
+        y = gather_elements(view, from, o, x.head, d, p.dim, elem);
+        if (!wide) {
+          const uint4 hi = gather_elements(view, from, o, x.head, d + 8, p.dim, elem);
+          y.z = hi.x, y.w = hi.y;
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&m->kv_full[st]));
+      }
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)  // (registers have no index)
+        if (i == k) r[i] = y;
+    }
+  };
+  auto place = [&](uint32_t dst, int first, const uint4 *r) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const int row = row_of(first + k);
+      if (row >= kTile) continue;
+      const uint32_t at = dst + (row >> 3) * p.group_stride + (row & 7) * 128;
+      auto put = [&](int c, uint32_t a, uint32_t b, uint32_t e, uint32_t f) {
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + (c >> 3) * p.panel_stride + (((c & 7) ^ (row & 7)) << 4)), "r"(a),
+                     "r"(b), "r"(e), "r"(f)
+                     : "memory");
+      };
+      if (wide) {
+        put(piece, r[k].x, r[k].y, r[k].z, r[k].w);
+      } else {
+        const uint32_t from[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+        uint32_t y[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t lo, hi;
+          asm("{ .reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b; }"
+              : "=r"(lo), "=r"(hi)
+              : "r"(from[q]));
+          y[2 * q] = T::from_f16x2(lo), y[2 * q + 1] = T::from_f16x2(hi);
+        }
+        put(2 * piece, y[0], y[1], y[2], y[3]);
+        put(2 * piece + 1, y[4], y[5], y[6], y[7]);
       }
     }
-    left -= stop - w.off;
-    if (left > 0) next_tile(p, w);
-  }
-  if (warp == 0) {
-    const uint32_t slot = item % kItems;
-    if (item >= kItems && !warp_wait(smem_addr(&m->item_empty[slot]), (item / kItems - 1) & 1)) return;
-    if (lane == 0) {
-      m->items[slot].rows = 0;
-      mbar_arrive(smem_addr(&m->item_full[slot]));
+  };
+
+#pragma unroll 1
+  for (uint32_t item = 0;; ++item) {
+    const Piece x = schedule.next(p);
+    if (warp == 0 && !publish<kDp>(p, qmap, x, item, base, m, elected, queries)) return;
+    if (x.rows == 0) break;
+    const TileOrder order = tile_order<S::kStreams>(p, x);
+    const int entries = 2 * S::kUnits * order.count;
+    uint4 ahead[kSteps];
+    if (entries > 0) fetch(x, order, 0, 0, ahead);
+#pragma unroll 1
+    for (int n = 0; n < entries; ++n) {
+      Ring<kDp> &ring = rings[n / S::kUnits & 1];
+      const uint32_t st = ring.slot();
+      uint4 now[kSteps];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) now[k] = ahead[k];
+      if (n + 1 < entries) fetch(x, order, n + 1, 0, ahead);
+      if (ring.entry >= S::kRing && !warp_wait(smem_addr(&m->kv_empty[st]), ring.phase() ^ 1)) return;
+      const uint32_t dst = ring.addr();
+      place(dst, 0, now);
+      if (wide) {  // twice as many loads: the others without looking ahead
+        fetch(x, order, n, kSteps, now);
+        place(dst, kSteps, now);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&m->kv_full[st]));
+      ++ring.entry;
     }
   }
 #pragma unroll 1
@@ -1007,13 +1072,144 @@ __device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, ui
   }
 }
 
-// ---- products -----
+// e4m3 pages by TMA: one warp loads the bytes of an entry's rows as they are into a small ring, six
+// warps turn them into operand rows of the query's type (exact).  K and V of a tile, then the next
+// tile's.  Against warps that fetch the bytes themselves this takes look-ups, addresses and the
+// memory's latency off the converting warps: 16 x 128 new tokens over 1000 to 4000 cached ones in
+// 444 us that way.
+template <int kDp>
+__device__ void load_role_raw(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, const CUtensorMap *qmap, uint32_t base,
+                              Misc *m) {
+  using S = Shape<kDp>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t elected = elect_lane();
+  uint32_t queries[2] = {0, 0};
+  uint32_t entry = 0;
+  const int boxes = kTile / p.box;
+  const bool head_inner = p.head_inner != 0;
+  Schedule schedule(p);
+#pragma unroll 1
+  for (uint32_t item = 0;; ++item) {
+    const Piece x = schedule.next(p);
+    if (!publish<kDp>(p, qmap, x, item, base, m, elected, queries)) break;
+    if (__all_sync(0xFFFFFFFFu, x.rows == 0)) break;
+    const TileOrder order = tile_order<S::kStreams>(p, x);
+    bool ok = true;
+    int32_t page = p.num_blocks, in_page = 0;
+#pragma unroll 1
+    for (int q = -1; q < order.count && ok; ++q) {
+      const int32_t now_page = page, now_in = in_page;
+      const int32_t tok = order.tile(min(q + 1, order.count - 1)) * kTile + lane * p.box;
+      page = p.num_blocks, in_page = 0;
+      if (lane < boxes && tok < x.q.len) {
+        const int32_t b = page_of(p, x.seq, tok);
+        if (b >= 0) page = b;
+        in_page = p.bs_shift >= 0 ? tok & (p.block_size - 1) : tok % p.block_size;
+      }
+      if (q < 0) continue;
+#pragma unroll 1
+      for (int n = 0; n < 2 * S::kUnits && ok; ++n, ++entry) {
+        const uint32_t st = entry & 1;
+        if (entry >= 2 && !warp_wait(smem_addr(&m->raw_empty[st]), (entry >> 1 & 1) ^ 1)) {
+          ok = false;
+          break;
+        }
+        const int u = n % S::kUnits;
+        const uint32_t bar = smem_addr(&m->raw_full[st]);
+        uint32_t dst = base + S::kRawAt + st * S::kRawBytes;
+        if (elected) mbar_expect_tx(bar, S::kRawBytes);
+        __syncwarp();
+#pragma unroll 1
+        for (int k = 0; k < boxes; ++k, dst += p.box * S::kUnitPanels * 64) {
+          const int32_t pg = __shfl_sync(0xFFFFFFFFu, now_page, k), in = __shfl_sync(0xFFFFFFFFu, now_in, k);
+          tma_load4(elected, dst, n >= S::kUnits ? vmap : kmap, u * S::kUnitPanels * 64, head_inner ? x.head : in, head_inner ? in : x.head, pg,
+                    bar);
+        }
+      }
+    }
+    if (!ok) break;
+  }
+  // what is in flight arrives before the CTA ends
+#pragma unroll 1
+  for (uint32_t n = entry - min(entry, 2u); n != entry; ++n) warp_wait(smem_addr(&m->raw_full[n & 1]), n >> 1 & 1);
+}
+
+template <typename T, int kDp>
+__device__ void convert_role(const ChunkParams &p, char *smem, uint32_t base, Misc *m) {
+  using S = Shape<kDp>;
+  constexpr int kPieces = S::kUnitPanels * 4;                                 // 16-byte pieces of a row
+  constexpr int kSteps = (4 * kPieces + kConvertWarps - 1) / kConvertWarps;  // of a lane and entry
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) - (kMmaWarp + 2);
+  const uint32_t elected = elect_lane();
+  const int piece = lane % kPieces, in_group = lane / kPieces;
+  Ring<kDp> rings[2] = {Ring<kDp>(base, 0), Ring<kDp>(base, 1)};
+  uint32_t entry = 0;
+#pragma unroll 1
+  for (uint32_t item = 0;; ++item) {
+    Piece x;
+    if (!receive(m, item, elected, &x)) return;
+    if (__all_sync(0xFFFFFFFFu, x.rows == 0)) break;
+    const TileOrder order = tile_order<S::kStreams>(p, x);
+#pragma unroll 1
+    for (int n = 0; n < order.count * 2 * S::kUnits; ++n, ++entry) {
+      const int valid = x.q.len - order.tile(n / (2 * S::kUnits)) * kTile;  // rows behind the sequence become zeros
+      Ring<kDp> &ring = rings[n / S::kUnits & 1];
+      const uint32_t st = entry & 1;
+      if (!warp_wait(smem_addr(&m->raw_full[st]), entry >> 1 & 1)) return;
+      const char *raw = smem + S::kRawAt + st * S::kRawBytes;
+      uint4 r[kSteps];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int row = (warp + kConvertWarps * k) * (32 / kPieces) + in_group;
+        r[k] = make_uint4(0, 0, 0, 0);
+        if (row < min(valid, kTile)) r[k] = *reinterpret_cast<const uint4 *>(raw + row * (kPieces * 16) + piece * 16);
+      }
+      __syncwarp();
+      if (elected) mbar_arrive(smem_addr(&m->raw_empty[st]));
+      if (ring.entry >= S::kRing && !warp_wait(smem_addr(&m->kv_empty[ring.slot()]), ring.phase() ^ 1)) return;
+      const uint32_t dst = ring.addr();
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int row = (warp + kConvertWarps * k) * (32 / kPieces) + in_group;
+        const uint32_t from[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
+        uint32_t y[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t lo, hi;
+          asm("{ .reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b; }"
+              : "=r"(lo), "=r"(hi)
+              : "r"(from[q]));
+          y[2 * q] = T::from_f16x2(lo), y[2 * q + 1] = T::from_f16x2(hi);
+        }
+        if (row >= kTile) continue;
+        const uint32_t at = dst + (row >> 3) * p.group_stride + (row & 7) * 128 + (2 * piece >> 3) * p.panel_stride;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at + ((((2 * piece + c) & 7) ^ (row & 7)) << 4)), "r"(y[4 * c]),
+                       "r"(y[4 * c + 1]), "r"(y[4 * c + 2]), "r"(y[4 * c + 3])
+                       : "memory");
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (elected) mbar_arrive(smem_addr(&m->kv_full[ring.slot()]));
+      ++ring.entry;
+    }
+  }
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {  // releases that are still to arrive
+    Ring<kDp> &ring = rings[k];
+    const uint32_t held = min(ring.entry, static_cast<uint32_t>(S::kRing)), last = ring.entry;
+    for (ring.entry = last - held; ring.entry != last; ++ring.entry)
+      if (!warp_wait(smem_addr(&m->kv_empty[ring.slot()]), ring.phase())) return;
+  }
+}
+
+// ---- products -----------------------------------------------------------------------------
 //
 // A tcgen05.commit that follows another one waits in the issuing warp until the products ahead of the
 // first have ended (about 800 clocks here), so there is one commit per group of products: scores
 // announce themselves and with them every product issued earlier.  What else waits for the products
 // -- the rings, the query tile -- is told by the softmax warps.
-//------------------------------------------------------------------------
 
 template <typename T, int kDp>
 struct Products {
@@ -1593,8 +1789,8 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
 //   + whole boxes, two loading warps, converged issue, one commit per product     1200   1110 - 1220
 // Two warps per 32 rows (half the columns each, 640 threads) ran at 1470 and 1340; keeping all 128
 // scores of a row in registers at 1440 and 1320; strict turns between the streams changed nothing.
-template <typename T, int kDp, bool kTma>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int kDp, Loads kLoads>
+__global__ void __launch_bounds__(kLoads == kTmaLoads ? 384 : 512, 1)  // = threads_of(kLoads)
     kvx_chunk_attention_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                                const __grid_constant__ CUtensorMap qmap) {
   using S = Shape<kDp>;
@@ -1607,13 +1803,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kItems; ++i) {
       mbar_init(smem_addr(&m->item_full[i]), 1);
-      mbar_init(smem_addr(&m->item_empty[i]), S::kStreams * 4 + (kTma ? 2 : 1));  // softmax warps, products, V loads
+      mbar_init(smem_addr(&m->item_empty[i]), S::kStreams * 4 + (kLoads == kTmaLoads ? 2 : kLoads == kRawLoads ? 1 + kConvertWarps : 1));  // softmax, products, others
     }
     for (int i = 0; i < 2 * S::kRing; ++i) {
-      mbar_init(smem_addr(&m->kv_full[i]), kTma ? 1 : 3);
+      mbar_init(smem_addr(&m->kv_full[i]), kLoads == kTmaLoads ? 1 : kLoads == kRawLoads ? kConvertWarps : kCopyWarps);
       mbar_init(smem_addr(&m->kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&m->raw_full[i]), 1);
+      mbar_init(smem_addr(&m->raw_empty[i]), kConvertWarps);
       mbar_init(smem_addr(&m->q_full[i]), p.q_tma ? 1 : 4);
       mbar_init(smem_addr(&m->q_empty[i]), 1);
       mbar_init(smem_addr(&m->s_full[i]), 1);
@@ -1656,8 +1854,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_commit(pr.elected, smem_addr(&m->drain));
       mbar_wait(smem_addr(&m->drain), 0);
       __syncwarp();
-    } else if (kTma) {
+    } else if (kLoads == kTmaLoads) {
       if (warp <= kMmaWarp + 2) load_role_tma<kDp>(p, &kmap, &vmap, &qmap, base, m, warp == kMmaWarp + 2);
+    } else if (kLoads == kRawLoads) {
+      if (warp == kMmaWarp + 1)
+        load_role_raw<kDp>(p, &kmap, &vmap, &qmap, base, m);
+      else
+        convert_role<T, kDp>(p, smem, base, m);
     } else {
       load_role_copy<T, kDp>(p, &qmap, base, m);
     }
@@ -1946,6 +2149,22 @@ bool make_map(CUtensorMap *map, const ChunkParams &p, const PageView &v, bool bf
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// e4m3 pages: (dim, head and token in the order of their strides, page), rows of one entry's dims.
+bool make_raw_map(CUtensorMap *map, const ChunkParams &p, const PageView &v, int unit_panels) {
+  const EncodeTiled encode = encode_tiled();
+  if (encode == nullptr) return false;
+  const cuuint64_t heads = static_cast<cuuint64_t>(p.heads_kv), toks = static_cast<cuuint64_t>(p.block_size);
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.dim), p.head_inner ? heads : toks, p.head_inner ? toks : heads,
+                              static_cast<cuuint64_t>(p.num_blocks)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(p.head_inner ? v.head : v.tok), static_cast<cuuint64_t>(p.head_inner ? v.tok : v.head),
+                                 static_cast<cuuint64_t>(v.blk)};
+  const cuuint32_t rows = static_cast<cuuint32_t>(p.box);
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(unit_panels * 64), p.head_inner ? 1 : rows, p.head_inner ? rows : 1, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, v.base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // What a head adds to the coordinates of whole boxes; false when K or V does not fold that way.
 bool fold_heads(ChunkParams *p) {
   if (p->dim % 64 != 0) return false;
@@ -1975,27 +2194,27 @@ bool make_query_map(CUtensorMap *map, const ChunkParams &p, bool bf16) {
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool tma_strides(const PageView &v) {
+bool tma_strides(const PageView &v, int64_t elem) {
   const int64_t most = int64_t{1} << 40;
-  return v.pack == 1 && v.dhi == 2 && aligned16(v.base) && v.blk % 16 == 0 && v.tok % 16 == 0 && v.head % 16 == 0 && v.blk > 0 &&
+  return v.pack == 1 && v.dhi == elem && aligned16(v.base) && v.blk % 16 == 0 && v.tok % 16 == 0 && v.head % 16 == 0 && v.blk > 0 &&
          v.tok > 0 && v.head > 0 && v.blk < most && v.tok < most && v.head < most;
 }
 
-template <typename T, int kDp, bool kTma>
+template <typename T, int kDp, Loads kLoads>
 void launch_tensor(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, const CUtensorMap &q, cudaStream_t st) {
   const size_t smem = chunk_smem_bytes<kDp>();
   // (the attribute is per device and cheap to set, so it is set on every launch)
-  cudaFuncSetAttribute(kvx_chunk_attention_kernel<T, kDp, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  launch_pdl(kvx_chunk_attention_kernel<T, kDp, kTma>, dim3(static_cast<unsigned>(p.grid)), kThreads, smem, st, p, k, v, q);
+  cudaFuncSetAttribute(kvx_chunk_attention_kernel<T, kDp, kLoads>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_pdl(kvx_chunk_attention_kernel<T, kDp, kLoads>, dim3(static_cast<unsigned>(p.grid)), static_cast<unsigned>(threads_of(kLoads)), smem, st, p, k, v, q);
 }
-template <typename T, bool kTma>
+template <typename T, Loads kLoads>
 void launch_tensor_dim(const ChunkParams &p, const CUtensorMap &k, const CUtensorMap &v, const CUtensorMap &q, cudaStream_t st) {
   if (p.dim <= 64)
-    launch_tensor<T, 64, kTma>(p, k, v, q, st);
+    launch_tensor<T, 64, kLoads>(p, k, v, q, st);
   else if (p.dim <= 128)
-    launch_tensor<T, 128, kTma>(p, k, v, q, st);
+    launch_tensor<T, 128, kLoads>(p, k, v, q, st);
   else
-    launch_tensor<T, 256, kTma>(p, k, v, q, st);
+    launch_tensor<T, 256, kLoads>(p, k, v, q, st);
 }
 template <int kDb>
 void launch_simt(const ChunkParams &p, cudaStream_t st) {
@@ -2120,10 +2339,12 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
     const int unit_panels = D <= 64 ? 1 : 2;
     const bool bf16 = io == KVX_DTYPE_BF16;
     p.head_inner = p.k.head < p.k.tok ? 1 : 0;
-    bool tma = elem == 2 && p.box >= 8 && tma_strides(p.k) && tma_strides(p.v) && (p.k.head < p.k.tok) == (p.v.head < p.v.tok);
+    const bool strides = tma_strides(p.k, elem) && tma_strides(p.v, elem) && (p.k.head < p.k.tok) == (p.v.head < p.v.tok);
+    bool tma = elem == 2 && p.box >= 8 && strides;
     p.whole_boxes = tma && fold_heads(&p) ? 1 : 0;
     if (p.whole_boxes && !(make_map(&kmap, p, p.k, bf16, unit_panels) && make_map(&vmap, p, p.v, bf16, unit_panels))) p.whole_boxes = 0;
     if (tma && !p.whole_boxes) tma = make_map(&kmap, p, p.k, bf16, unit_panels) && make_map(&vmap, p, p.v, bf16, unit_panels);
+    const bool raw = elem == 1 && p.box >= 8 && strides && make_raw_map(&kmap, p, p.k, unit_panels) && make_raw_map(&vmap, p, p.v, unit_panels);
     p.group_stride = p.whole_boxes ? unit_panels * 1024 : 1024;
     p.panel_stride = p.whole_boxes ? 1024 : kPanelBytes;
     CUtensorMap qmap = {};
@@ -2131,23 +2352,23 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
                       make_query_map(&qmap, p, io == KVX_DTYPE_BF16)
                   ? 1
                   : 0;
-    const int64_t piece = 8 * elem;  // bytes one lane copies at a time where TMA is not used
-    auto rows_ok = [&](const PageView &v) {
-      return v.pack == 1 && v.dhi == elem && reinterpret_cast<uintptr_t>(v.base) % piece == 0 && v.blk % piece == 0 && v.tok % piece == 0 &&
-             v.head % piece == 0;
+    auto rows_ok = [&](const PageView &v) {  // rows that 16-byte loads can read where TMA is not used
+      return v.pack == 1 && v.dhi == elem && aligned16(v.base) && v.blk % 16 == 0 && v.tok % 16 == 0 && v.head % 16 == 0;
     };
-    p.kv_vec = D % 8 == 0 && rows_ok(p.k) && rows_ok(p.v) ? 1 : 0;
-    if (io == KVX_DTYPE_BF16) {
+    p.kv_vec = D * elem % 16 == 0 && rows_ok(p.k) && rows_ok(p.v) ? 1 : 0;
+    auto launch = [&](auto type) {
+      using T = decltype(type);
       if (tma)
-        launch_tensor_dim<Bf16, true>(p, kmap, vmap, qmap, cs);
+        launch_tensor_dim<T, kTmaLoads>(p, kmap, vmap, qmap, cs);
+      else if (raw)
+        launch_tensor_dim<T, kRawLoads>(p, kmap, vmap, qmap, cs);
       else
-        launch_tensor_dim<Bf16, false>(p, kmap, vmap, qmap, cs);
-    } else {
-      if (tma)
-        launch_tensor_dim<Fp16, true>(p, kmap, vmap, qmap, cs);
-      else
-        launch_tensor_dim<Fp16, false>(p, kmap, vmap, qmap, cs);
-    }
+        launch_tensor_dim<T, kCopyLoads>(p, kmap, vmap, qmap, cs);
+    };
+    if (bf16)
+      launch(Bf16{});
+    else
+      launch(Fp16{});
   } else if (D <= 64) {
     launch_simt<64>(p, cs);
   } else if (D <= 128) {

@@ -64,6 +64,7 @@ struct ChunkParams {
   int32_t whole_boxes;         // 1: a box carries all panels of its tokens, [8 tokens][panel]; 0: one panel
   int32_t head_panels, head_groups;  // whole boxes: what a head adds to the panel and the group coordinate
   int32_t head_inner;          // else: heads are closer together than tokens
+  int32_t plan_inside;         // 1: few sequences, planned by the attention kernel itself
   int32_t q_tma;               // 1: query tiles are loaded by TMA
   int32_t q_vec;               // 1: query rows can be read, out rows written in 16-byte pieces
   int32_t kv_vec;              // 1: page rows can be read in 16-byte pieces
@@ -131,10 +132,55 @@ __device__ __forceinline__ int32_t steps_of(const ChunkParams &p, const Seq &q, 
   return max(1, n) + p.tile_cost;
 }
 
-constexpr int kPlanThreads = 1024;
+// Steps of one sequence over all KV heads, for every lane's own; the lanes of a warp help each other
+// with sequences of many tiles.
+__device__ __forceinline__ int64_t sequence_steps(const ChunkParams &p, int s) {
+  const int lane = threadIdx.x & 31;
+  Seq q{0, 0, 0, 0};
+  int32_t tiles = 0;
+  if (s < p.seq_count) {
+    q = load_seq(p, s);
+    tiles = tiles_of(p, q);
+  }
+  int64_t mine = 0;
+  if (tiles <= 8)
+    for (int t = 0; t < tiles; ++t) mine += steps_of(p, q, t);
+  unsigned big = __ballot_sync(0xFFFFFFFFu, tiles > 8);
+  while (big != 0) {
+    const int from = __ffs(big) - 1;
+    big &= big - 1;
+    Seq x;
+    x.first = 0;
+    x.rows = __shfl_sync(0xFFFFFFFFu, q.rows, from);
+    x.len = __shfl_sync(0xFFFFFFFFu, q.len, from);
+    x.pos0 = __shfl_sync(0xFFFFFFFFu, q.pos0, from);
+    const int32_t nt = tiles_of(p, x);
+    int64_t sum = 0;
+    for (int t = lane; t < nt; t += 32) sum += steps_of(p, x, t);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    if (lane == from) mine = sum;
+  }
+  return mine * p.heads_kv;
+}
 
-// prefix[s] = steps of the sequences ahead of s, over all KV heads.  One warp per sequence adds up
-// its tiles, then one scan over the warps' sums.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanInside = 32;  // up to that many sequences every CTA makes the plan itself
+
+// prefix[s] = steps of the sequences ahead of s, for at most kPlanInside sequences; one warp.
+__device__ void plan_few(const ChunkParams &p, int64_t *prefix) {
+  const int lane = threadIdx.x & 31;
+  int64_t incl = sequence_steps(p, lane);
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t y = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 0) prefix[0] = 0;
+  if (lane < p.seq_count) prefix[lane + 1] = incl;
+}
+
+// The same for any number.
 __global__ void __launch_bounds__(kPlanThreads) kvx_chunk_plan_kernel(const ChunkParams p) {
   pdl_prologue();
   __shared__ int64_t s_sum[32];
@@ -143,34 +189,8 @@ __global__ void __launch_bounds__(kPlanThreads) kvx_chunk_plan_kernel(const Chun
   if (threadIdx.x == 0) s_base = 0;
   __syncthreads();
   for (int s0 = 0; s0 < p.seq_count; s0 += kPlanThreads) {
-    // a thread adds up its own sequence when it has few tiles, a warp joins for the others
     const int s = s0 + threadIdx.x;
-    Seq q{0, 0, 0, 0};
-    int32_t tiles = 0;
-    if (s < p.seq_count) {
-      q = load_seq(p, s);
-      tiles = tiles_of(p, q);
-    }
-    int64_t mine = 0;
-    if (tiles <= 8)
-      for (int t = 0; t < tiles; ++t) mine += steps_of(p, q, t);
-    unsigned big = __ballot_sync(0xFFFFFFFFu, tiles > 8);
-    while (big != 0) {
-      const int from = __ffs(big) - 1;
-      big &= big - 1;
-      Seq x;
-      x.first = 0;
-      x.rows = __shfl_sync(0xFFFFFFFFu, q.rows, from);
-      x.len = __shfl_sync(0xFFFFFFFFu, q.len, from);
-      x.pos0 = __shfl_sync(0xFFFFFFFFu, q.pos0, from);
-      const int32_t nt = tiles_of(p, x);
-      int64_t sum = 0;
-      for (int t = lane; t < nt; t += 32) sum += steps_of(p, x, t);
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-      if (lane == from) mine = sum;
-    }
-    mine *= p.heads_kv;
+    const int64_t mine = sequence_steps(p, s);
     int64_t incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -211,21 +231,21 @@ __device__ __forceinline__ int64_t snap(const ChunkParams &p, int64_t at, int64_
 }
 
 // All lanes of a warp call it together and get the same answer.  `at` < prefix[seq_count].
-__device__ Place find_place(const ChunkParams &p, int64_t at) {
+__device__ Place find_place(const ChunkParams &p, const int64_t *prefix, int64_t at) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = p.seq_count;  // the last s with prefix[s] <= at lies in [lo, hi)
   while (hi - lo > 1) {
     const int step = max(1, (hi - lo + 31) / 32);
     const int s = lo + lane * step;
-    const unsigned in = __ballot_sync(0xFFFFFFFFu, s < hi && p.prefix[s] <= at);
+    const unsigned in = __ballot_sync(0xFFFFFFFFu, s < hi && prefix[s] <= at);
     lo = lo + (31 - __clz(in)) * step;
     hi = min(hi, lo + step);
   }
   Place w;
   w.seq = lo;
   w.q = load_seq(p, lo);
-  const int64_t in_seq = at - p.prefix[lo];
-  const int64_t per_head = (p.prefix[lo + 1] - p.prefix[lo]) / p.heads_kv;
+  const int64_t in_seq = at - prefix[lo];
+  const int64_t per_head = (prefix[lo + 1] - prefix[lo]) / p.heads_kv;
   w.head = static_cast<int32_t>(in_seq / per_head);
   int64_t left = in_seq - w.head * per_head;
   const int32_t nt = tiles_of(p, w.q);
@@ -254,8 +274,8 @@ __device__ Place find_place(const ChunkParams &p, int64_t at) {
 }
 
 // Share `share` of the schedule: from `w` on, `left` steps.
-__device__ __forceinline__ int64_t find_share(const ChunkParams &p, int share, Place *w) {
-  const int64_t total = p.prefix[p.seq_count];
+__device__ __forceinline__ int64_t find_share(const ChunkParams &p, const int64_t *prefix, int share, Place *w) {
+  const int64_t total = prefix[p.seq_count];
   const int n = shares(p, total);
   if (share >= n) return 0;
   int64_t at[2];
@@ -264,7 +284,7 @@ __device__ __forceinline__ int64_t find_share(const ChunkParams &p, int share, P
   for (int i = 0; i < 2; ++i) {
     at[i] = share_begin(total, n, share + i);
     if (at[i] >= total) continue;
-    e[i] = find_place(p, at[i]);
+    e[i] = find_place(p, prefix, at[i]);
     const int64_t begin = at[i] - e[i].off, to = snap(p, at[i], begin, begin + e[i].steps);
     e[i].off = static_cast<int32_t>(to - begin);
     at[i] = to;
@@ -383,7 +403,7 @@ __global__ void __launch_bounds__(kMergeThreads) kvx_chunk_merge_kernel(const Ch
   const int cut = blockIdx.x + 1;
   if (cut >= n) return;
   const int64_t raw = share_begin(total, n, cut);
-  const Place w = find_place(p, raw);
+  const Place w = find_place(p, p.prefix, raw);
   const int64_t tile_at = raw - w.off, tile_end = tile_at + w.steps;
   const int64_t at = snap(p, raw, tile_at, tile_end);
   if (at == tile_at || at == tile_end) return;
@@ -667,6 +687,7 @@ struct Misc {
   uint64_t raw_full[2], raw_empty[2];
   uint64_t tail, drain;
   Piece items[kItems];
+  int64_t prefix[kPlanInside + 1];
   float join_m[kTile], join_l[kTile];
   uint32_t tmem;
 };
@@ -758,8 +779,8 @@ struct Ring {
 struct Schedule {
   Place w;
   int64_t left;
-  __device__ __forceinline__ explicit Schedule(const ChunkParams &p) {
-    left = find_share(p, blockIdx.x, &w);
+  __device__ __forceinline__ Schedule(const ChunkParams &p, const int64_t *prefix) {
+    left = find_share(p, prefix, blockIdx.x, &w);
     if (left > 0 && w.off >= w.steps) next_tile(p, w);
   }
   __device__ __forceinline__ Piece next(const ChunkParams &p) {
@@ -884,7 +905,7 @@ __device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, con
     return true;
   };
   bool ok = true;
-  Schedule schedule(p);
+  Schedule schedule(p, p.plan_inside ? m->prefix : p.prefix);
 #pragma unroll 1
   for (uint32_t item = 0; ok; ++item) {
     Piece x;
@@ -950,7 +971,7 @@ __device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, ui
   Ring<kDp> rings[2] = {Ring<kDp>(base, 0), Ring<kDp>(base, 1)};
   uint32_t queries[2] = {0, 0};
   const uint32_t elected = elect_lane();
-  Schedule schedule(p);
+  Schedule schedule(p, p.plan_inside ? m->prefix : p.prefix);
   const bool wide = p.cache_code != KVX_DTYPE_F8_E4M3;  // 16-bit elements
   const int elem = wide ? 2 : 1, pieces = wide ? 2 * kPieces : kPieces;
   const int in_group = lane / pieces, piece = lane % pieces;
@@ -1087,7 +1108,7 @@ __device__ void load_role_raw(const ChunkParams &p, const CUtensorMap *kmap, con
   uint32_t entry = 0;
   const int boxes = kTile / p.box;
   const bool head_inner = p.head_inner != 0;
-  Schedule schedule(p);
+  Schedule schedule(p, p.plan_inside ? m->prefix : p.prefix);
 #pragma unroll 1
   for (uint32_t item = 0;; ++item) {
     const Piece x = schedule.next(p);
@@ -1829,11 +1850,16 @@ __global__ void __launch_bounds__(kLoads == kTmaLoads ? 384 : 512, 1)  // = thre
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&m->tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.plan_inside && warp == 0) {
+    plan_few(p, m->prefix);
+    // (the merge kernel reads it, too)
+    if (blockIdx.x == 0) plan_few(p, p.prefix);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = m->tmem;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp < kMmaWarp) {
     if (S::kStreams == 2 || warp < 4) softmax_role<T, kDp>(p, base, smem, tmem, m);
@@ -1895,7 +1921,7 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int share = blockIdx.x;
   Place w;
-  int64_t left = find_share(p, share, &w);
+  int64_t left = find_share(p, p.prefix, share, &w);
   if (left > 0 && w.off >= w.steps) next_tile(p, w);
   const int io = elem_bytes(p.io_code);
   while (left > 0) {
@@ -2052,6 +2078,7 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 struct Split {
   int32_t tile_rows, kv_tile, grid, slot_rows, min_share, tile_cost;
+  bool cuts;  // whether tiles may be cut
   size_t prefix_bytes, ml_bytes, o_bytes;
   size_t total() const { return prefix_bytes + ml_bytes + o_bytes; }
 };
@@ -2073,7 +2100,9 @@ Split split_of(bool tensor, int64_t seqs, int64_t rows, int64_t heads_q, int64_t
   s.grid = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(most, (steps + s.min_share - 1) / s.min_share)));
   s.slot_rows = static_cast<int32_t>(std::min<int64_t>(s.tile_rows, rows * group));
   s.prefix_bytes = (static_cast<size_t>(seqs + 1) * sizeof(int64_t) + 15) / 16 * 16;
-  const size_t slots = s.grid > 1 ? static_cast<size_t>(2) * s.grid * s.slot_rows : 0;
+  // (a cut that would leave a tile of at most two steps in two parts goes to its edge: see snap)
+  s.cuts = s.grid > 1 && per_tile - s.tile_cost > 2;
+  const size_t slots = s.cuts ? static_cast<size_t>(2) * s.grid * s.slot_rows : 0;
   s.ml_bytes = slots * 2 * sizeof(float);
   s.o_bytes = slots * dim * sizeof(float);
   return s;
@@ -2327,7 +2356,8 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   p.q_vec = D % 8 == 0 && p.q_pitch % 16 == 0 && p.o_pitch % 16 == 0 && aligned16(p.query) && aligned16(p.out) ? 1 : 0;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
 
-  launch_pdl(kvx_chunk_plan_kernel, dim3(1), static_cast<unsigned>(kPlanThreads), size_t{0}, cs, p);
+  p.plan_inside = tensor && S <= kPlanInside ? 1 : 0;
+  if (!p.plan_inside) launch_pdl(kvx_chunk_plan_kernel, dim3(1), static_cast<unsigned>(kPlanThreads), size_t{0}, cs, p);
   if (tensor) {
     p.box = 1;
     while (p.box < kTile && p.block_size % (2 * p.box) == 0) p.box *= 2;
@@ -2380,7 +2410,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   } else {
     launch_simt<1024>(p, cs);
   }
-  if (p.grid > 1) {
+  if (sp.cuts) {
     const unsigned y = static_cast<unsigned>(std::max(1, std::min(16, p.slot_rows / 16)));
     launch_pdl(kvx_chunk_merge_kernel, dim3(static_cast<unsigned>(p.grid - 1), y), static_cast<unsigned>(kMergeThreads), size_t{0}, cs, p);
   }

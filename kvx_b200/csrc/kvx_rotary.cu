@@ -44,6 +44,8 @@ struct RotaryParams {
   int32_t num_blocks, block_size, fp8;
   int32_t q_in_place, k_in_place;  // what is not turned need not be copied
   int32_t tile;                    // tokens per CTA
+  // vector tier: units of a head and V vectors of one, with their shifts (-1: no power of two)
+  int32_t units, units_shift, v_units, v_shift;
 };
 
 __device__ __forceinline__ int64_t read_index(const void *p, int64_t i, int wide) {
@@ -162,7 +164,7 @@ __device__ __forceinline__ void pdl_prologue() {
 
 // ------------------------------------------------------------------ vector tier --------
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxTile = 16;
 
 template <typename T, bool kInterleaved>
@@ -185,9 +187,9 @@ __global__ void __launch_bounds__(kThreads) kvx_rotary_kernel(const RotaryParams
 
   // units of a head: the vectors (or pairs of vectors) that are turned, then those that are not
   const int turned = kInterleaved ? 2 * p.half / kVec : p.half / kVec;
-  const int units = turned + (p.dim - 2 * p.half) / kVec;
+  const int units = p.units;
   const int heads = p.q_heads + p.k_heads;             // turned heads of a token
-  const int v_units = paged ? p.k_heads * (p.dim / kVec) : 0;
+  const int v_units = paged ? p.k_heads * p.v_units : 0;
   const int per_token = heads * units + v_units;
   for (int i = threadIdx.x; i < n * per_token; i += kThreads) {
     const int t = i / per_token;
@@ -197,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) kvx_rotary_kernel(const RotaryParams
       const SlotAt at = sm_slot[t];
       if (at.block < 0) continue;
       rest -= heads * units;
-      const int h = rest / (p.dim / kVec), d = (rest - h * (p.dim / kVec)) * kVec;
+      const int h = p.v_shift >= 0 ? rest >> p.v_shift : rest / p.v_units, d = (rest - h * p.v_units) * kVec;
       const uint4 x = load_stream(p.v + tok * p.v_pitch + (static_cast<int64_t>(h) * p.dim + d) * kE);
       char *to = p.vc.base + at.block * p.vc.blk + at.off * p.vc.tok + h * p.vc.head;
       if (!p.fp8) {
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) kvx_rotary_kernel(const RotaryParams
       }
       continue;
     }
-    const int h = rest / units, u = rest - h * units;
+    const int h = p.units_shift >= 0 ? rest >> p.units_shift : rest / units, u = rest - h * units;
     const bool is_k = h >= p.q_heads;
     const int kh = h - p.q_heads;
     const bool pass = u >= turned;
@@ -399,10 +401,16 @@ kvx_status_t launch(RotaryParams &p, cudaStream_t st) {
                    rows16(p.k_out, p.ko_pitch) && (!paged || (rows16(p.v, p.v_pitch) && pages16(p.kc) && pages16(p.vc))) &&
                    static_cast<int64_t>(p.q_heads + 2 * p.k_heads) * p.dim <= (1 << 22) && p.half <= 1024;
   if (vec) {
-    // tokens per CTA: enough that the angles' latency is spread, few enough that small batches
-    // still occupy the machine
-    p.tile = 4;
+    // Tokens per CTA: the angles' latency is hidden by the other CTAs of the SM, so small CTAs do
+    // best.  16 384 tokens of 32 + 8 heads x 128 with the write of K and V (389 MB), us: 66.6 with 2
+    // tokens and 128 threads (5.8 TB/s, 89 % of a copy), 67.7 / 4 / 256, 69.8 / 2 / 256, 72.1 / 8 / 256;
+    // two or four units in flight per thread 75 and 101 (registers cost more CTAs than they bring loads).
+    p.tile = 2;
     while (p.tile > 1 && (p.tokens + p.tile - 1) / p.tile < 148 * 4) p.tile >>= 1;
+    auto shift_of = [](int32_t x) { return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(x)) : -1; };
+    p.units = (p.interleaved ? 2 * p.half : p.half) / kVec + (p.dim - 2 * p.half) / kVec;
+    p.v_units = p.dim / kVec;
+    p.units_shift = shift_of(p.units), p.v_shift = shift_of(p.v_units);
     const unsigned grid = static_cast<unsigned>((p.tokens + p.tile - 1) / p.tile);
     const size_t smem = static_cast<size_t>(p.tile) * p.half * 2 * sizeof(float);
     if (p.interleaved)

@@ -81,8 +81,8 @@ KVX_API kvx_status_t kvx_launch_paged_attention_decode(const kvx_cache_desc_t *c
  *
  * over the cached tokens t < min(seq_lens[s], max_seq_len) that the table resolves (as above), for
  * causal = 1 only those with t <= the row's position.  A row that sees no token, or whose scores
- * are all -inf, gets out = 0.  A token that is not seen has no influence, whatever its page
- * holds.  n may differ from sequence to sequence and may be 0 or exceed seq_lens[s] (rows at
+ * are all -inf, gets out = 0.  A token that is not seen has no influence beyond the rounding of
+ * the weights, whatever its page holds.  n may differ from sequence to sequence and may be 0 or exceed seq_lens[s] (rows at
  * negative positions see nothing).  Rows at or beyond `rows`, rows of a sequence with a negative
  * query_indptr, and rows that belong to no sequence stay untouched.  Scores, softmax and sums are
  * f32; on the tensor-core path the softmax weights are rounded once to the query's type before
@@ -115,7 +115,7 @@ KVX_API size_t kvx_paged_attention_chunk_workspace_bytes(uint32_t seq_count, uin
                                                          uint32_t num_q_heads, uint32_t num_kv_heads,
                                                          uint32_t head_dim, uint32_t max_seq_len);
 
-/* Enqueues the attention on `stream` (2 or 3 kernels) and returns without synchronising.  Cache
+/* Enqueues the attention on `stream` (1 to 3 kernels) and returns without synchronising.  Cache
  * types, layouts and scales as for kvx_launch_paged_attention_decode; head_dim up to 1024 (up to
  * 256 with a 16-bit query on the tensor cores).  Calls that may overlap on the GPU need scratch of
  * their own.

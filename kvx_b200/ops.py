@@ -533,7 +533,7 @@ def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     slot are turned but not cached."""
     if query_out is None:
         query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    native = native_ops() if key_cache.dim() == 4 else None
+    native = native_ops() if key_cache.dim() == 4 and query.is_cuda else None
     if native is not None:
         dev = query.device
         _call_native(native.rotary_and_cache, query, key, value, positions, inv_freq, key_cache, value_cache, slot_mapping,

@@ -850,6 +850,7 @@ __device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, con
   };
   auto load_piece = [&](const Piece &x) {
     const TileOrder order = tile_order<S::kStreams>(p, x);
+    if (order.count == 0) return true;  // no tile, and so none whose pages could be looked up ahead
     const int32_t c_panel = x.head * p.head_panels, c_group = x.head * p.head_groups;
     int32_t in_page = 0, page = p.num_blocks;
 #pragma unroll 1
@@ -1115,6 +1116,7 @@ __device__ void load_role_raw(const ChunkParams &p, const CUtensorMap *kmap, con
     if (!publish<kDp>(p, qmap, x, item, base, m, elected, queries)) break;
     if (__all_sync(0xFFFFFFFFu, x.rows == 0)) break;
     const TileOrder order = tile_order<S::kStreams>(p, x);
+    if (order.count == 0) continue;  // no tile, and so none whose pages could be looked up ahead
     bool ok = true;
     int32_t page = p.num_blocks, in_page = 0;
 #pragma unroll 1

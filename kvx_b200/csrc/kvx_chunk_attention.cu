@@ -2196,9 +2196,11 @@ bool make_raw_map(CUtensorMap *map, const ChunkParams &p, const PageView &v, int
                 CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// What a head adds to the coordinates of whole boxes; false when K or V does not fold that way.
-bool fold_heads(ChunkParams *p) {
-  if (p->dim % 64 != 0) return false;
+// What a head adds to the coordinates of whole boxes; false when K or V does not fold that way.  A
+// box must not reach behind its head (head_dim 192 in two boxes of 128): the next head's values are
+// not zeros there, and zero queries times its infinities would be NaN.
+bool fold_heads(ChunkParams *p, int unit_panels) {
+  if (p->dim % (64 * unit_panels) != 0) return false;
   p->head_panels = p->head_groups = 0;
   if (p->heads_kv == 1) return true;
   const PageView &k = p->k, &v = p->v;
@@ -2373,7 +2375,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
     p.head_inner = p.k.head < p.k.tok ? 1 : 0;
     const bool strides = tma_strides(p.k, elem) && tma_strides(p.v, elem) && (p.k.head < p.k.tok) == (p.v.head < p.v.tok);
     bool tma = elem == 2 && p.box >= 8 && strides;
-    p.whole_boxes = tma && fold_heads(&p) ? 1 : 0;
+    p.whole_boxes = tma && fold_heads(&p, unit_panels) ? 1 : 0;
     if (p.whole_boxes && !(make_map(&kmap, p, p.k, bf16, unit_panels) && make_map(&vmap, p, p.v, bf16, unit_panels))) p.whole_boxes = 0;
     if (tma && !p.whole_boxes) tma = make_map(&kmap, p, p.k, bf16, unit_panels) && make_map(&vmap, p, p.v, bf16, unit_panels);
     const bool raw = elem == 1 && p.box >= 8 && strides && make_raw_map(&kmap, p, p.k, unit_panels) && make_raw_map(&vmap, p, p.v, unit_panels);

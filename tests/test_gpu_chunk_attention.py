@@ -367,3 +367,23 @@ def test_more_sequences_than_the_plan_scans_at_once():
     n = torch.randint(0, 3, (2500,), generator=g).tolist()
     t = torch.randint(0, 60, (2500,), generator=g).tolist()
     check(make(lens=tuple(zip(n, t)), kv_heads=1, group=2, dim=64, seed=6, block_size=32))
+
+
+@pytest.mark.parametrize("cache", ["same", "f8"])
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+@pytest.mark.parametrize("dim", [64, 80, 96, 128, 192, 256])
+def test_heads_do_not_touch_each_other(dim, layout, cache):
+    """NaN all over the K and V of every other head: the heads between keep their bits."""
+    torch, _ = _torch()
+    c = make(dim=dim, layout=layout, cache=cache, kv_heads=4, group=2, lens=((70, 300), (3, 40)), seed=15)
+    clean = check(c)
+    for name in ("kc", "vc"):
+        x = c[name].view(torch.uint8) if cache == "f8" else c[name]
+        for h in (1, 3):
+            (x[:, :, h] if layout == "nhd" else x[:, h]).fill_(0x7F if cache == "f8" else math.nan)
+    out = run(c, dim ** -0.5)
+    kept, lost = out.unflatten(1, (4, 2))[:, [0, 2]], out.unflatten(1, (4, 2))[:, [1, 3]]
+    same = torch.equal(kept, clean.unflatten(1, (4, 2))[:, [0, 2]])
+    assert same
+    all_nan = bool(lost.isnan().all())
+    assert all_nan

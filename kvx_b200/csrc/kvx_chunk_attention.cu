@@ -94,12 +94,13 @@ struct Seq {
 
 __device__ __forceinline__ Seq load_seq(const ChunkParams &p, int s) {
   const int64_t a = read_index(p.indptr, s, p.indptr64);
-  int64_t b = read_index(p.indptr, s + 1, p.indptr64);
-  if (b > p.rows) b = p.rows;
-  const int64_t n = (a < 0 || b <= a) ? 0 : b - a;
+  const int64_t b = read_index(p.indptr, s + 1, p.indptr64);
   int64_t len = read_index(p.lens, s, p.table64);
   if (len < 0) len = 0;
-  const int64_t pos0 = len - n;
+  const bool none = a < 0 || b <= a || a >= p.rows;
+  // (rows behind the last are left out, the others keep their positions)
+  const int64_t n = none ? 0 : min(b, static_cast<int64_t>(p.rows)) - a;
+  const int64_t pos0 = none ? 0 : max(len - (b - a), static_cast<int64_t>(INT32_MIN));
   len = min(len, static_cast<int64_t>(p.max_seq_len));
   len = min(len, static_cast<int64_t>(p.max_blocks) * p.block_size);
   Seq q;
@@ -112,13 +113,14 @@ __device__ __forceinline__ Seq load_seq(const ChunkParams &p, int s) {
 
 __device__ __forceinline__ int32_t row_limit(const ChunkParams &p, const Seq &q, int32_t r) {
   if (!p.causal) return q.len;
-  return max(0, min(q.len, q.pos0 + r / p.group + 1));
+  const int64_t end = static_cast<int64_t>(q.pos0) + r / p.group + 1;
+  return static_cast<int32_t>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(q.len), end)));
 }
 __device__ __forceinline__ int32_t tiles_of(const ChunkParams &p, const Seq &q) {
   return (q.rows + p.tile_rows - 1) / p.tile_rows;
 }
 __device__ __forceinline__ bool is_narrow(const ChunkParams &p, const Seq &q) {
-  return p.pair != 0 && q.rows * 2 <= p.tile_rows;
+  return p.pair != 0 && q.rows <= p.tile_rows / 2;
 }
 // K/V tiles and steps of row tile `t`.  A tile without any is still one step: its rows are written;
 // loading its queries and writing its result count as `tile_cost` steps ahead of the first.

@@ -387,3 +387,24 @@ def test_heads_do_not_touch_each_other(dim, layout, cache):
     assert same
     all_nan = bool(lost.isnan().all())
     assert all_nan
+
+
+def test_rows_behind_the_query_keep_their_positions():
+    """query_indptr that names more rows than there are: those that exist are where they would be; the
+    same for lengths beyond 32 bits that max_seq_len cuts."""
+    torch, _ = _torch()
+    c = make(lens=((9, 40), (20, 90)), seed=16, indptr="i64")
+    full = check(c)
+    c["q"] = c["q"][:17]
+    out = run(c, c["dim"] ** -0.5)
+    same = torch.equal(out, full[:17])
+    assert same
+    c["indptr"][2] = 2 ** 40  # the sequence's tokens lie far ahead of its length: none sees anything
+    out = run(c, c["dim"] ** -0.5)
+    assert torch.equal(out[:9], full[:9]) and not bool(out[9:].any())
+    c = make(lens=((9, 40), (20, 90)), seed=16, index="i64")
+    c["lens"][1] = 2 ** 40  # every new token is behind max_seq_len and sees all of it
+    out = run(c, c["dim"] ** -0.5, max_seq_len=90)
+    want, tol = expected(c, c["dim"] ** -0.5, causal=False)
+    worst = float(((out[9:].double() - want[9:]).abs() - tol[9:]).max())
+    assert worst <= 0

@@ -81,13 +81,15 @@ KVX_API kvx_status_t kvx_launch_paged_attention_decode(const kvx_cache_desc_t *c
  *
  * over the cached tokens t < min(seq_lens[s], max_seq_len) that the table resolves (as above), for
  * causal = 1 only those with t <= the row's position.  A row that sees no token, or whose scores
- * are all -inf, gets out = 0.  A token that is not seen has no influence beyond the rounding of
- * the weights, whatever its page holds.  n may differ from sequence to sequence and may be 0 or exceed seq_lens[s] (rows at
- * negative positions see nothing).  Rows at or beyond `rows`, rows of a sequence with a negative
- * query_indptr, and rows that belong to no sequence stay untouched.  Scores, softmax and sums are
- * f32; on the tensor-core path the softmax weights are rounded once to the query's type before
- * they multiply V (a relative error of half a unit in the last place of that type, of the order
- * of the output's own rounding); the result is rounded once to the query's type. */
+ * are all -inf, gets out = 0.  A token that is not seen has no influence beyond the rounding of the
+ * weights, whatever its page holds.  n may differ from sequence to sequence and may be 0 or exceed
+ * seq_lens[s] (rows at negative positions see nothing).  Rows at or beyond `rows`, rows of a
+ * sequence with a negative query_indptr, and rows that belong to no sequence stay untouched.  The
+ * row ranges of the sequences must not overlap, and out must not overlap query (query rows are
+ * read after others were written).  Scores, softmax and sums are f32; on the tensor-core path the
+ * softmax weights are rounded once to the query's type before they multiply V (a relative error of
+ * half a unit in the last place of that type, of the order of the output's own rounding); the
+ * result is rounded once to the query's type. */
 typedef struct kvx_chunk_attention_desc {
   uint32_t size;
   uint32_t num_q_heads;    /* a multiple of cache->num_kv_heads */
@@ -121,11 +123,12 @@ KVX_API size_t kvx_paged_attention_chunk_workspace_bytes(uint32_t seq_count, uin
  * their own.
  *
  * Status: INVALID_ARGUMENT for NULL / undersized descriptors, shapes that disagree, a query head
- * count that is not a multiple of the KV heads, causal above 1, scratch smaller than
- * kvx_paged_attention_chunk_workspace_bytes() or misaligned (16 bytes); UNSUPPORTED for a table
- * that is not PACKED, mismatched types, token rows with gaps between or inside heads, rows that
- * overlap, more than 2^31 - 1024 rows x (num_q_heads / num_kv_heads), head_dim above 1024; OK
- * without a launch when there is no sequence or no row. */
+ * count that is not a multiple of the KV heads, causal above 1, out at the query's address,
+ * max_seq_len above 2^31 - 1025, scratch smaller than kvx_paged_attention_chunk_workspace_bytes()
+ * or misaligned (16 bytes); UNSUPPORTED for a table that is not PACKED, mismatched types, token
+ * rows with gaps between or inside heads, rows that overlap, more than 2^31 - 1024 rows x
+ * (num_q_heads / num_kv_heads), head_dim above 1024; OK without a launch when there is no sequence
+ * or no row. */
 KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *cache,
                                                       const kvx_chunk_attention_desc_t *attn,
                                                       const kvx_scale_desc_t *k_scale,

@@ -2311,7 +2311,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   if (st != KVX_STATUS_OK) return st;
   if (attn->query.data == nullptr || attn->out.data == nullptr || attn->query_indptr == nullptr ||
       attn->block_table.indices == nullptr || attn->seq_lens.lengths == nullptr || cache->k.data == nullptr ||
-      cache->v.data == nullptr || attn->block_table.max_blocks_per_seq == 0 ||
+      cache->v.data == nullptr || attn->block_table.max_blocks_per_seq == 0 || attn->query.data == attn->out.data ||
       attn->block_table.max_blocks_per_seq > static_cast<uint32_t>(INT32_MAX) || cache->num_blocks > static_cast<uint32_t>(INT32_MAX) ||
       cache->block_size > static_cast<uint32_t>(INT32_MAX) || attn->max_seq_len > static_cast<uint32_t>(INT32_MAX) - 1024u ||
       S > INT32_MAX || D > INT32_MAX)

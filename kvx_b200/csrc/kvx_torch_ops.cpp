@@ -362,6 +362,7 @@ void paged_attention_chunk(torch::Tensor &out, const torch::Tensor &query, const
   describe_cache(&cache, key_cache, value_cache, kv_cache_dtype, kv_heads, dim);
   if (max_seq_len <= 0)
     max_seq_len = std::min<int64_t>(block_table.size(1) * static_cast<int64_t>(cache.block_size), INT32_MAX - 2048);
+  TORCH_CHECK(max_seq_len <= INT32_MAX - 1024, "max_seq_len is too large");
   a.size = sizeof(a);
   a.num_q_heads = static_cast<uint32_t>(query.size(1));
   a.max_seq_len = static_cast<uint32_t>(max_seq_len);

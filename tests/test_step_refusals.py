@@ -8,6 +8,7 @@ from kvx_b200 import abi
 
 OK, INVALID, UNSUPPORTED = abi.STATUS_OK, abi.STATUS_INVALID_ARGUMENT, abi.STATUS_UNSUPPORTED
 FAKE = 0x10000  # a non-NULL "device" address that is never dereferenced on these paths
+OUT = 0x20000   # another one
 
 
 def cache(dtype=abi.DTYPE_BF16, layout=abi.LAYOUT_NHD, pack=1, dim=64):
@@ -30,7 +31,7 @@ def mutated(desc, **kw):
 # ---------------------------------------------------------------- chunk attention
 
 def chunk(**kw):
-    return mutated(abi.chunk_attention_desc(3, 10, 8, 64, abi.DTYPE_BF16, FAKE, FAKE, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE,
+    return mutated(abi.chunk_attention_desc(3, 10, 8, 64, abi.DTYPE_BF16, FAKE, OUT, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE,
                                             abi.DTYPE_S32, FAKE), **kw)
 
 
@@ -51,7 +52,7 @@ def test_chunk_attention_refusals(built_lib):
     for kw in (dict(size=8), dict(num_q_heads=7), dict(num_q_heads=0), dict(max_seq_len=0), dict(causal=2), dict(block_table__size=4),
                dict(seq_lens__size=4), dict(seq_lens__seq_count=2), dict(seq_lens__dtype=abi.DTYPE_S64), dict(query__shape__1=6),
                dict(query__shape__2=32), dict(out__shape__0=9), dict(query__ndim=2), dict(query__size=8),
-               dict(query_indptr_dtype=abi.DTYPE_U32), dict(query_indptr=None), dict(query__data=None), dict(out__data=None),
+               dict(query_indptr_dtype=abi.DTYPE_U32), dict(query_indptr=None), dict(query__data=None), dict(out__data=None), dict(out__data=FAKE),
                dict(block_table__indices=None), dict(seq_lens__lengths=None), dict(block_table__max_blocks_per_seq=0),
                dict(max_seq_len=2 ** 31)):
         assert attend(L, cache(), chunk(**kw)) == INVALID, kw
@@ -64,14 +65,14 @@ def test_chunk_attention_refusals(built_lib):
     assert attend(L, c, chunk()) == INVALID
     assert attend(L, cache(abi.DTYPE_F8_E4M3), chunk(), scales=False) == UNSUPPORTED
     assert attend(L, mutated(cache(), k__layout=abi.LAYOUT_CUSTOM, v__layout=abi.LAYOUT_CUSTOM), chunk()) == UNSUPPORTED
-    wide = abi.chunk_attention_desc(3, 10, 8, 1100, abi.DTYPE_BF16, FAKE, FAKE, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE, abi.DTYPE_S32, FAKE)
+    wide = abi.chunk_attention_desc(3, 10, 8, 1100, abi.DTYPE_BF16, FAKE, OUT, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE, abi.DTYPE_S32, FAKE)
     assert attend(L, cache(dim=1100), wide) == UNSUPPORTED
-    many = abi.chunk_attention_desc(3, 2 ** 30, 8, 64, abi.DTYPE_BF16, FAKE, FAKE, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE, abi.DTYPE_S32, FAKE)
+    many = abi.chunk_attention_desc(3, 2 ** 30, 8, 64, abi.DTYPE_BF16, FAKE, OUT, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE, abi.DTYPE_S32, FAKE)
     assert attend(L, cache(), many) == UNSUPPORTED  # 2^30 rows x 4 heads
     # nothing to do
     none = abi.chunk_attention_desc(3, 0, 8, 64, abi.DTYPE_BF16, 0, 0, 0.1, True, 64, abi.DTYPE_S32, FAKE, 4, FAKE, abi.DTYPE_S32, FAKE)
     assert attend(L, cache(), none, None, 0) == OK
-    none = abi.chunk_attention_desc(0, 5, 8, 64, abi.DTYPE_BF16, FAKE, FAKE, 0.1, True, 64, abi.DTYPE_S32, 0, 4, 0, abi.DTYPE_S32, FAKE)
+    none = abi.chunk_attention_desc(0, 5, 8, 64, abi.DTYPE_BF16, FAKE, OUT, 0.1, True, 64, abi.DTYPE_S32, 0, 4, 0, abi.DTYPE_S32, FAKE)
     assert attend(L, cache(), none, None, 0) == OK
 
 

@@ -10,7 +10,7 @@ from . import abi
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libkvx_b200.so")
 _lib = None
 
-# Every symbol include/kvx_abi.h, the headers under include/ declare.
+# Every symbol the headers under include/ declare.
 EXPORTS = [
     "kvx_get_version", "kvx_validate_cache_desc", "kvx_write_kv", "kvx_gather_kv",
     "kvx_launch_write_kv", "kvx_launch_write_kv_prefill", "kvx_launch_gather_kv",

@@ -829,7 +829,7 @@ __device__ __forceinline__ bool receive(Misc *m, uint32_t item, uint32_t elected
 // its tokens where the layout allows, its coordinates are looked up a tile ahead, one box per lane,
 // and the boxes are issued by one lane of converged code.
 template <int kDp>
-__device__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, const CUtensorMap *qmap, uint32_t base,
+__device__ __forceinline__ void load_role_tma(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, const CUtensorMap *qmap, uint32_t base,
                               Misc *m, bool mine_v) {
   using S = Shape<kDp>;
   const int lane = threadIdx.x & 31;
@@ -966,7 +966,7 @@ __device__ __noinline__ uint4 gather_elements(const PageView &view, const char *
 // flight while the one before it is converted.  Each warp walks the schedule for itself, the first
 // one publishes the pieces.
 template <typename T, int kDp>
-__device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, uint32_t base, Misc *m) {
+__device__ __forceinline__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, uint32_t base, Misc *m) {
   using S = Shape<kDp>;
   constexpr int kPieces = S::kUnitPanels * 4;  // 16-byte pieces of a row of e4m3 (twice as many of 16-bit elements)
   constexpr int kSteps = (4 * kPieces + kCopyWarps - 1) / kCopyWarps;  // loads of a lane and entry (twice as many ..)
@@ -1102,7 +1102,7 @@ __device__ void load_role_copy(const ChunkParams &p, const CUtensorMap *qmap, ui
 // memory's latency off the converting warps: 16 x 128 new tokens over 1000 to 4000 cached ones in
 // 444 us that way.
 template <int kDp>
-__device__ void load_role_raw(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, const CUtensorMap *qmap, uint32_t base,
+__device__ __forceinline__ void load_role_raw(const ChunkParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, const CUtensorMap *qmap, uint32_t base,
                               Misc *m) {
   using S = Shape<kDp>;
   const int lane = threadIdx.x & 31;
@@ -1160,7 +1160,7 @@ __device__ void load_role_raw(const ChunkParams &p, const CUtensorMap *kmap, con
 }
 
 template <typename T, int kDp>
-__device__ void convert_role(const ChunkParams &p, char *smem, uint32_t base, Misc *m) {
+__device__ __forceinline__ void convert_role(const ChunkParams &p, char *smem, uint32_t base, Misc *m) {
   using S = Shape<kDp>;
   constexpr int kPieces = S::kUnitPanels * 4;                                 // 16-byte pieces of a row
   constexpr int kSteps = (4 * kPieces + kConvertWarps - 1) / kConvertWarps;  // of a lane and entry
@@ -1455,7 +1455,7 @@ __device__ __forceinline__ void correct_scores(const ChunkParams &p, const Piece
 }
 
 template <typename T, int kDp>
-__device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, uint32_t tmem0, Misc *m) {
+__device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, uint32_t tmem0, Misc *m) {
   using S = Shape<kDp>;
   const int s = threadIdx.x >> 7;                 // stream
   const int tid = threadIdx.x & 127, lane = threadIdx.x & 31;
@@ -1541,9 +1541,26 @@ __device__ void softmax_role(const ChunkParams &p, uint32_t base, char *smem, ui
     const int32_t limit = tid < rows ? row_limit(p, x.q, row_at + tid) : INT32_MAX;
     float mx = -INFINITY, l = 0.f;
     const uint32_t o_at = tmem0 + lanes + 256 + s * kDp;
+    int from = b;
+    if ((tid & ~31) >= rows) {
+      // All rows of this warp lie behind the tile's last: no weights to make.  What the products do
+      // with its lanes stays in its lanes.  (A loop of its own: the same as a branch in the loop below
+      // made that one a fifth slower.)
+#pragma unroll 1
+      for (; from < e; ++from, ++tiles) {
+        const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
+        if (!warp_wait(smem_addr(&m->s_full[0]) + 8 * buf, (S::kScoreBufs == 2 ? tiles >> 1 : tiles) & 1)) return;
+        if (S::kStreams == 1 && from > b && !warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
+        if (lane == 0) {
+          mbar_arrive(smem_addr(&m->p_part[0]) + 8 * buf);
+          mbar_arrive(smem_addr(&m->p_full[0]) + 8 * buf);
+        }
+        __syncwarp();
+      }
+    }
     bool page_ok = pages_exist(p, x, b * kTile);
 #pragma unroll 1
-    for (int j = b; j < e; ++j, ++tiles) {
+    for (int j = from; j < e; ++j, ++tiles) {
       const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
       const uint32_t ph = (S::kScoreBufs == 2 ? tiles >> 1 : tiles) & 1;
       const uint32_t s_at = tmem0 + lanes + buf * kTile;

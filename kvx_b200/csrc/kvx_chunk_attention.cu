@@ -2086,6 +2086,206 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
   }
 }
 
+// f32 caches whose rows 16-byte copies can read, head_dim up to 256, more than 32 rows per sequence: steps
+// of 64 rows x 64 tokens, bound by the FMA units.  A thread has 4 rows x 4 tokens of the scores and 4 rows x
+// kDb / 16 dims of the output; the 16 lanes that share rows are half a warp, so weights pass through shared
+// memory without a barrier of the CTA.  K and V have a buffer each, filled asynchronously: the next K while
+// the softmax and the output product run, the next V while the next scores do.
+constexpr int kWideRows = 64, kWideTokens = 64;
+constexpr size_t wide_smem_bytes(int bucket) {
+  return (static_cast<size_t>(kWideRows + 2 * kWideTokens) * (bucket + 4) + kWideRows * (kWideTokens + 4) + 2 * kWideTokens) * sizeof(float);
+}
+
+__device__ __forceinline__ void copy16_async(uint32_t to, const char *from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+template <int kDb>  // head_dim (a multiple of 4) rounded up to 64, 128 or 256
+__global__ void __launch_bounds__(kSimtThreads, kDb > 64 ? 1 : 2) kvx_chunk_attention_f32_kernel(const ChunkParams p) {
+  constexpr int kPitch = kDb + 4, kPitchP = kWideTokens + 4, kCols = kDb / 64;
+  extern __shared__ float4 sm_wide[];
+  float *sm_q = reinterpret_cast<float *>(sm_wide);  // [64][kPitch]
+  float *sm_k = sm_q + kWideRows * kPitch;            // [64][kPitch]
+  float *sm_v = sm_k + kWideTokens * kPitch;          // [64][kPitch]
+  float *sm_p = sm_v + kWideTokens * kPitch;          // [64][kPitchP]
+  int32_t *sm_page = reinterpret_cast<int32_t *>(sm_p + kWideRows * kPitchP);  // [2][64]: of this tile and the next
+  pdl_prologue();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ty = tid >> 4, tx = tid & 15;
+  const int quads = p.dim / 4;
+  Place w;
+  int64_t left = find_share(p, p.prefix, blockIdx.x, &w);
+  if (left > 0 && w.off >= w.steps) next_tile(p, w);
+#pragma unroll 1
+  while (left > 0) {
+    const int32_t stop = static_cast<int32_t>(min(static_cast<int64_t>(w.steps), w.off + left));
+    const Piece x = piece_of(p, w, stop, blockIdx.x);
+    const float mul = nonzero(score_mul(p, x.head)), am = fabsf(mul);
+    auto look_up = [&](int j) { return j < x.kv1 && j * kWideTokens + tid < x.q.len ? page_of(p, x.seq, j * kWideTokens + tid) : -1; };
+    auto fetch = [&](const PageView &view, float *to, int j) {  // tokens without a page become zeros
+      const int32_t *pages = sm_page + (j & 1) * kWideTokens;
+#pragma unroll 4
+      for (int i = tid; i < kWideTokens * quads; i += kSimtThreads) {
+        const int c = i / quads, d = (i - c * quads) * 4;
+        const int32_t page = pages[c], tok = j * kWideTokens + c;
+        const int32_t o = p.bs_shift >= 0 ? tok & (p.block_size - 1) : tok % p.block_size;
+        const char *from = page < 0 ? view.base : view.base + page * view.blk + o * view.tok + x.head * view.head + d * 4;
+        copy16_async(smem_addr(to + c * kPitch + d), from, page >= 0);
+      }
+    };
+    __syncthreads();  // the previous piece is done with shared memory
+    if (tid < kWideTokens) sm_page[(x.kv0 & 1) * kWideTokens + tid] = look_up(x.kv0);
+    for (int row = warp; row < kWideRows; row += kSimtThreads / 32) {
+      const int32_t r = x.row0 + row, token = r / p.group, h = x.head * p.group + (r - token * p.group);
+      const float *from = reinterpret_cast<const float *>(p.query + (x.q.first + token) * p.q_pitch) + static_cast<int64_t>(h) * p.dim;
+      for (int d = lane; d < p.dim; d += 32) {
+        const float y = row < x.rows ? from[d] : 0.f;
+        sm_q[row * kPitch + d] = mul < 0.f ? -y : y;
+      }
+    }
+    __syncthreads();
+    if (x.kv0 < x.kv1) fetch(p.k, sm_k, x.kv0);
+    copies_commit();
+    if (x.kv0 < x.kv1) fetch(p.v, sm_v, x.kv0);
+    copies_commit();
+    float acc[4][kCols][4], m[4], l[4];
+    int32_t limit[4];  // (rows behind the tile's last are never written: nothing is masked for them)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      m[a] = -INFINITY, l[a] = 0.f;
+      limit[a] = ty * 4 + a < x.rows ? row_limit(p, x.q, x.row0 + ty * 4 + a) : INT32_MAX;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[a][c][e] = 0.f;
+    }
+    const bool works = (warp * 8) < x.rows;  // warps without rows only load
+    const int32_t least = min(min(limit[0], limit[1]), min(limit[2], limit[3]));
+#pragma unroll 1
+    for (int j = x.kv0; j < x.kv1; ++j) {
+      const int32_t t0 = j * kWideTokens;
+      const int32_t next_page = tid < kWideTokens ? look_up(j + 1) : -1;
+      copies_wait<1>();
+      __syncthreads();  // K of this tile is there
+      float s[4][4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) s[a][b] = 0.f;
+      if (works) {
+#pragma unroll 2
+        for (int d = 0; d < p.dim; d += 4) {
+          float4 q[4], k[4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) q[a] = *reinterpret_cast<const float4 *>(&sm_q[(ty * 4 + a) * kPitch + d]);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) k[b] = *reinterpret_cast<const float4 *>(&sm_k[(tx + 16 * b) * kPitch + d]);
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              s[a][b] = fmaf(q[a].w, k[b].w, fmaf(q[a].z, k[b].z, fmaf(q[a].y, k[b].y, fmaf(q[a].x, k[b].x, s[a][b]))));
+        }
+      }
+      if (tid < kWideTokens) sm_page[((j + 1) & 1) * kWideTokens + tid] = next_page;
+      __syncthreads();  // K is free, the next tile's pages are known
+      if (j + 1 < x.kv1) fetch(p.k, sm_k, j + 1);
+      copies_commit();
+      if (works) {
+        bool there[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) there[b] = sm_page[(j & 1) * kWideTokens + tx + 16 * b] >= 0;
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < 4; ++b)
+            if (there[b] && t0 + tx + 16 * b < limit[a]) top = fmaxf(top, s[a][b]);
+#pragma unroll
+          for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+          const float mn = fmaxf(m[a], top), c = weight_of(m[a], mn, am);
+          float sum = 0.f;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            float y = 0.f;
+            if (there[b] && t0 + tx + 16 * b < limit[a])
+              y = mn == -INFINITY ? (s[a][b] == s[a][b] ? 0.f : s[a][b]) : exp2f((s[a][b] - mn) * am);
+            sum += y;
+            sm_p[(ty * 4 + a) * kPitchP + tx + 16 * b] = y;
+          }
+          l[a] = l[a] * c + sum;  // of this lane's tokens
+          m[a] = mn;
+#pragma unroll
+          for (int e = 0; e < kCols; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[a][e][i] *= c;
+        }
+      }
+      copies_wait<1>();
+      __syncthreads();  // V of this tile and the weights are there
+      if (works) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < kWideTokens; c0 += 4) {
+          float wv[4][4];
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const float4 y = *reinterpret_cast<const float4 *>(&sm_p[(ty * 4 + a) * kPitchP + c0]);
+            wv[a][0] = y.x, wv[a][1] = y.y, wv[a][2] = y.z, wv[a][3] = y.w;
+          }
+          const bool all = t0 + c0 + 3 < least;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              const float4 v = *reinterpret_cast<const float4 *>(&sm_v[(c0 + t) * kPitch + c * 64 + tx * 4]);
+#pragma unroll
+              for (int a = 0; a < 4; ++a) {
+                if (!all && t0 + c0 + t >= limit[a]) continue;  // left out, not weighted with zero
+                acc[a][c][0] = fmaf(wv[a][t], v.x, acc[a][c][0]);
+                acc[a][c][1] = fmaf(wv[a][t], v.y, acc[a][c][1]);
+                acc[a][c][2] = fmaf(wv[a][t], v.z, acc[a][c][2]);
+                acc[a][c][3] = fmaf(wv[a][t], v.w, acc[a][c][3]);
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();  // V is free
+      if (j + 1 < x.kv1) fetch(p.v, sm_v, j + 1);
+      copies_commit();
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) l[a] += __shfl_xor_sync(0xFFFFFFFFu, l[a], d);
+      const int row = ty * 4 + a;
+      if (row >= x.rows) continue;
+      const int32_t r = x.row0 + row, token = r / p.group, h = x.head * p.group + (r - token * p.group);
+      float *out = reinterpret_cast<float *>(p.out + (x.q.first + token) * p.o_pitch) + static_cast<int64_t>(h) * p.dim;
+      const int64_t part = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + row;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = c * 64 + tx * 4 + i;
+          if (d >= p.dim) continue;
+          if (x.slot >= 0)
+            p.part_o[part * p.dim + d] = acc[a][c][i];
+          else
+            out[d] = l[a] == 0.f ? 0.f : acc[a][c][i] / l[a];
+        }
+      }
+      if (x.slot >= 0 && tx == 0) reinterpret_cast<float2 *>(p.part_ml)[part] = make_float2(m[a], l[a]);
+    }
+    left -= stop - w.off;
+    if (left > 0) next_tile(p, w);
+  }
+}
+
 // ------------------------------------------------------------------ host ---------------
 
 constexpr int kMaxShares = 148;      // of the tensor-core kernel: one CTA per SM
@@ -2097,6 +2297,9 @@ constexpr int kSimtTileCost = 1;
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// The tensor-core kernel, the f32 kernel of large steps, the one for everything else.
+enum Family { kTensor, kWide, kSimt };
+
 struct Split {
   int32_t tile_rows, kv_tile, grid, slot_rows, min_share, tile_cost;
   bool cuts;  // whether tiles may be cut
@@ -2106,14 +2309,15 @@ struct Split {
 
 // Scratch and shares of one kernel family.  Every share that begins or ends inside a tile has a
 // slot for it; there are never more shares than steps / min_share.
-Split split_of(bool tensor, int64_t seqs, int64_t rows, int64_t heads_q, int64_t heads_kv, int64_t dim, int64_t max_len) {
+Split split_of(Family family, int64_t seqs, int64_t rows, int64_t heads_q, int64_t heads_kv, int64_t dim, int64_t max_len) {
   Split s;
   const int64_t group = heads_q / heads_kv;
-  s.tile_rows = tensor ? (dim > 128 ? kTile : 2 * kTile) : kSimtRows;
-  s.kv_tile = tensor ? kTile : simt_tokens(static_cast<int>(dim > 512 ? 1024 : 64));
+  const bool tensor = family == kTensor;
+  s.tile_rows = tensor ? (dim > 128 ? kTile : 2 * kTile) : family == kWide ? kWideRows : kSimtRows;
+  s.kv_tile = tensor ? kTile : family == kWide ? kWideTokens : simt_tokens(static_cast<int>(dim > 512 ? 1024 : 64));
   s.min_share = tensor ? kMinShare : kMinSimtShare;
   s.tile_cost = tensor ? kTileCost : kSimtTileCost;
-  const int64_t most = tensor ? kMaxShares : (dim > 256 ? kMaxShares : kMaxSimtShares);
+  const int64_t most = tensor ? kMaxShares : family == kWide ? (dim > 64 ? kMaxShares : kMaxSimtShares) : (dim > 256 ? kMaxShares : kMaxSimtShares);
   const int64_t tiles = (seqs + rows * group / s.tile_rows) * heads_kv;
   const int64_t per_tile = std::max<int64_t>(1, (max_len + s.kv_tile - 1) / s.kv_tile) + s.tile_cost;
   int64_t steps;
@@ -2276,6 +2480,13 @@ void launch_simt(const ChunkParams &p, cudaStream_t st) {
   launch_pdl(kvx_chunk_attention_simt_kernel<kDb>, dim3(static_cast<unsigned>(p.grid)), kSimtThreads, smem, st, p);
 }
 
+template <int kDb>
+void launch_wide(const ChunkParams &p, cudaStream_t st) {
+  const size_t smem = wide_smem_bytes(kDb);
+  cudaFuncSetAttribute(kvx_chunk_attention_f32_kernel<kDb>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  launch_pdl(kvx_chunk_attention_f32_kernel<kDb>, dim3(static_cast<unsigned>(p.grid)), kSimtThreads, smem, st, p);
+}
+
 }  // namespace
 
 extern "C" {
@@ -2283,9 +2494,12 @@ extern "C" {
 KVX_API size_t kvx_paged_attention_chunk_workspace_bytes(uint32_t seq_count, uint32_t num_rows, uint32_t num_q_heads,
                                                          uint32_t num_kv_heads, uint32_t head_dim, uint32_t max_seq_len) {
   if (seq_count == 0 || num_rows == 0 || num_q_heads == 0 || num_kv_heads == 0 || num_q_heads < num_kv_heads || head_dim == 0) return 0;
-  const Split a = split_of(true, seq_count, num_rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
-  const Split b = split_of(false, seq_count, num_rows, num_q_heads, num_kv_heads, head_dim, max_seq_len);
-  return std::max(a.total(), b.total());
+  size_t most = 0;
+  for (const Family family : {kTensor, kWide, kSimt}) {
+    if (family != kSimt && head_dim > 256) continue;
+    most = std::max(most, split_of(family, seq_count, num_rows, num_q_heads, num_kv_heads, head_dim, max_seq_len).total());
+  }
+  return most;
 }
 
 KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *cache, const kvx_chunk_attention_desc_t *attn,
@@ -2338,7 +2552,14 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
 
   const bool tensor = io != KVX_DTYPE_F32 && D <= 256;
   if (!tensor && D > 1024) return KVX_STATUS_UNSUPPORTED;
-  const Split sp = split_of(tensor, S, R, Hq, H, D, attn->max_seq_len);
+  auto f32_rows = [](const PageView &v) {  // rows that 16-byte copies can read
+    return v.pack == 1 && v.dhi == 4 && aligned16(v.base) && v.blk % 16 == 0 && v.tok % 16 == 0 && v.head % 16 == 0;
+  };
+  const Family family = tensor                                                                        ? kTensor
+                        : cd == KVX_DTYPE_F32 && D <= 256 && D % 4 == 0 && f32_rows(p.k) && f32_rows(p.v) && R * group > kSimtRows * S
+                            ? kWide
+                            : kSimt;
+  const Split sp = split_of(family, S, R, Hq, H, D, attn->max_seq_len);
   const size_t need = kvx_paged_attention_chunk_workspace_bytes(static_cast<uint32_t>(S), static_cast<uint32_t>(R), attn->num_q_heads,
                                                                 cache->num_kv_heads, cache->head_dim, attn->max_seq_len);
   if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)) return KVX_STATUS_INVALID_ARGUMENT;
@@ -2422,6 +2643,13 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
       launch(Bf16{});
     else
       launch(Fp16{});
+  } else if (family == kWide) {
+    if (D <= 64)
+      launch_wide<64>(p, cs);
+    else if (D <= 128)
+      launch_wide<128>(p, cs);
+    else
+      launch_wide<256>(p, cs);
   } else if (D <= 64) {
     launch_simt<64>(p, cs);
   } else if (D <= 128) {

@@ -1918,12 +1918,12 @@ __global__ void __launch_bounds__(kLoads == kTmaLoads ? 384 : 512, 1)  // = thre
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// ------------------------------------------------------------------ f32 and everything else --
+// ------------------------------------------------------------------ everything else, f32 --
 //
-// f32 caches (and queries), head_dim above 256: the same schedule and the same one-pass softmax on
-// the f32 units.  A step is 32 rows x kN tokens: scores from shared memory, a warp owns 4 rows of
-// the softmax and of the output sums (a lane owns every 32nd dim), K and V share one buffer.
-
+// head_dim above 256, f32 with odd strides, HND_PACKED pages or an e4m3 cache: the same schedule and the
+// same one-pass softmax on the f32 units, every element read through the layout's rule.  A step is 32 rows
+// x kN tokens: scores from shared memory, a warp owns 4 rows of the softmax and of the output sums (a lane
+// owns every 32nd dim), K and V share one buffer.
 constexpr int kSimtThreads = 256;
 constexpr int kSimtRows = 32;
 constexpr int simt_tokens(int dim_bucket) { return dim_bucket > 512 ? 16 : 32; }
@@ -2086,11 +2086,13 @@ __global__ void __launch_bounds__(kSimtThreads) kvx_chunk_attention_simt_kernel(
   }
 }
 
-// f32 caches whose rows 16-byte copies can read, head_dim up to 256, more than 32 rows per sequence: steps
-// of 64 rows x 64 tokens, bound by the FMA units.  A thread has 4 rows x 4 tokens of the scores and 4 rows x
-// kDb / 16 dims of the output; the 16 lanes that share rows are half a warp, so weights pass through shared
-// memory without a barrier of the CTA.  K and V have a buffer each, filled asynchronously: the next K while
-// the softmax and the output product run, the next V while the next scores do.
+// f32 caches whose rows 16-byte copies can read, head_dim up to 256: steps of 64 rows x 64 tokens, bound by
+// the FMA units where the rows are many.  A thread has 4 rows x 4 tokens of the scores and 4 rows x kDb / 16
+// dims of the output; the 16 lanes that share rows are half a warp, so weights pass through shared memory
+// without a barrier of the CTA.  K and V have a buffer each, filled asynchronously: the next K while the
+// softmax and the output product run, the next V while the next scores do.  Against the kernel above, us:
+// 113 tokens x 16 heads over 5k-10k tokens of 4 heads x 64  2540 -> 586;  392 x 5 over 1.2k, 8 x 128  1231 -> 353;
+// with few rows, where the copies count:  8 x (1 token x 8 heads) over up to 6.6k, 8 x 128  1012 -> 262.
 constexpr int kWideRows = 64, kWideTokens = 64;
 constexpr size_t wide_smem_bytes(int bucket) {
   return (static_cast<size_t>(kWideRows + 2 * kWideTokens) * (bucket + 4) + kWideRows * (kWideTokens + 4) + 2 * kWideTokens) * sizeof(float);
@@ -2117,8 +2119,14 @@ __global__ void __launch_bounds__(kSimtThreads, kDb > 64 ? 1 : 2) kvx_chunk_atte
   pdl_prologue();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ty = tid >> 4, tx = tid & 15;
   const int quads = p.dim / 4;
+  __shared__ int64_t sm_prefix[kPlanInside + 1];
+  if (p.plan_inside) {
+    if (warp == 0) plan_few(p, sm_prefix);
+    if (warp == 0 && blockIdx.x == 0) plan_few(p, p.prefix);  // (the merge kernel reads it, too)
+    __syncthreads();
+  }
   Place w;
-  int64_t left = find_share(p, p.prefix, blockIdx.x, &w);
+  int64_t left = find_share(p, p.plan_inside ? sm_prefix : p.prefix, blockIdx.x, &w);
   if (left > 0 && w.off >= w.steps) next_tile(p, w);
 #pragma unroll 1
   while (left > 0) {
@@ -2556,7 +2564,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
     return v.pack == 1 && v.dhi == 4 && aligned16(v.base) && v.blk % 16 == 0 && v.tok % 16 == 0 && v.head % 16 == 0;
   };
   const Family family = tensor                                                                        ? kTensor
-                        : cd == KVX_DTYPE_F32 && D <= 256 && D % 4 == 0 && f32_rows(p.k) && f32_rows(p.v) && R * group > kSimtRows * S
+                        : cd == KVX_DTYPE_F32 && D <= 256 && D % 4 == 0 && f32_rows(p.k) && f32_rows(p.v)
                             ? kWide
                             : kSimt;
   const Split sp = split_of(family, S, R, Hq, H, D, attn->max_seq_len);
@@ -2600,7 +2608,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   p.q_vec = D % 8 == 0 && p.q_pitch % 16 == 0 && p.o_pitch % 16 == 0 && aligned16(p.query) && aligned16(p.out) ? 1 : 0;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
 
-  p.plan_inside = tensor && S <= kPlanInside ? 1 : 0;
+  p.plan_inside = family != kSimt && S <= kPlanInside ? 1 : 0;
   if (!p.plan_inside) launch_pdl(kvx_chunk_plan_kernel, dim3(1), static_cast<unsigned>(kPlanThreads), size_t{0}, cs, p);
   if (tensor) {
     p.box = 1;

@@ -408,3 +408,19 @@ def test_rows_behind_the_query_keep_their_positions():
     want, tol = expected(c, c["dim"] ** -0.5, causal=False)
     worst = float(((out[9:].double() - want[9:]).abs() - tol[9:]).max())
     assert worst <= 0
+
+
+@pytest.mark.parametrize("layout", ["nhd", "hnd"])
+@pytest.mark.parametrize("dim", [4, 60, 64, 100, 128, 192, 256])
+def test_f32_tiles(dim, layout):
+    """Full and ragged tiles of the f32 kernel, cut and whole, with pages that are missing."""
+    for i, (group, lens, causal) in enumerate([(1, ((1, 1), (64, 64), (65, 130)), True), (5, ((13, 300), (1, 700)), True),
+                                               (4, ((50, 200), (0, 9), (3, 2)), False)]):
+        check(make(dtype="f32", dim=dim, layout=layout, group=group, lens=lens, seed=20 + i, bad_pages=i, block_size=(16, 8, 20)[i]),
+              causal=causal)
+
+
+@pytest.mark.parametrize("layout,cache,dim", [("packed", "same", 64), ("nhd", "f8", 128), ("nhd", "same", 66), ("hnd", "f8", 80)])
+def test_f32_queries_over_other_pages(layout, cache, dim):
+    """What the f32 kernel's copies cannot read goes element by element."""
+    check(make(dtype="f32", cache=cache, dim=dim, layout=layout, group=2, lens=((40, 300), (1, 33)), seed=24))

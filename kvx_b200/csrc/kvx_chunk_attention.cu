@@ -960,7 +960,7 @@ __device__ __noinline__ uint4 gather_elements(const PageView &view, const char *
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Pages that TMA cannot read as operands (e4m3, HND_PACKED, odd page sizes, odd strides): seven warps
+// Pages that TMA cannot read (HND_PACKED, pages of less than 8 tokens, odd strides): seven warps
 // copy rows into the same swizzled tiles, converting on the way.  A warp's load instruction covers
 // whole rows in 16-byte pieces; pages are looked up a tile ahead, and the loads of an entry are in
 // flight while the one before it is converted.  Each warp walks the schedule for itself, the first
@@ -1544,8 +1544,7 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
     int from = b;
     if ((tid & ~31) >= rows) {
       // All rows of this warp lie behind the tile's last: no weights to make.  What the products do
-      // with its lanes stays in its lanes.  (A loop of its own: the same as a branch in the loop below
-      // made that one a fifth slower.)
+      // with its lanes stays in its lanes.
 #pragma unroll 1
       for (; from < e; ++from, ++tiles) {
         const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
@@ -1828,9 +1827,11 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
 // Measured on 16 prompts of 512 to 4096 tokens and on 4 x 512 tokens over 32k contexts (us):
 //   first version, one thread issuing everything, boxes issued by their lanes     2410   1310
 //   queries by TMA, column loops, waits that do not read the timer first          1290   1110 - 1250
-//   + whole boxes, two loading warps, converged issue, one commit per product     1200   1110 - 1220
-// Two warps per 32 rows (half the columns each, 640 threads) ran at 1470 and 1340; keeping all 128
-// scores of a row in registers at 1440 and 1320; strict turns between the streams changed nothing.
+//   + whole boxes, two loading warps, converged issue, one commit per product     1180   1080 - 1220
+// (824 and 950 TFLOP/s; behind other work, at the power cap, 1350 and 1250.)  64 x 5 drafted tokens over up to
+// 32k, bound by the loads: 226, 4.7 TB/s.  Two warps per 32 rows (half the columns each, 640 threads) ran
+// at 1470 and 1340; keeping all 128 scores of a row in registers at 1490 and 1390, the column loops
+// unrolled at 1440 and 1230; strict turns between the streams changed nothing.
 template <typename T, int kDp, Loads kLoads>
 __global__ void __launch_bounds__(kLoads == kTmaLoads ? 384 : 512, 1)  // = threads_of(kLoads)
     kvx_chunk_attention_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,

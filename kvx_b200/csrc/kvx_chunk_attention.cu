@@ -597,11 +597,6 @@ __device__ __forceinline__ void tc_st16(uint32_t at, const uint32_t *r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tc_st8(uint32_t at, const uint32_t *r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 // Shared-memory operand descriptor, 128-byte swizzle: rows of 128 bytes, 8 of them to an atom of
 // 1 024 bytes.  `stride` bytes between groups of 8 rows; `lead` bytes between blocks of 64
 // elements along the rows (used when the rows run along the reduction, i.e. for V).
@@ -2298,7 +2293,7 @@ __global__ void __launch_bounds__(kSimtThreads, kDb > 64 ? 1 : 2) kvx_chunk_atte
 // ------------------------------------------------------------------ host ---------------
 
 constexpr int kMaxShares = 148;      // of the tensor-core kernel: one CTA per SM
-constexpr int kMaxSimtShares = 296;  // of the f32 kernel
+constexpr int kMaxSimtShares = 296;  // of the kernels on the f32 units, where two CTAs share an SM
 constexpr int kMinShare = 2;         // steps; a shorter share costs more in its partial result than it saves
 constexpr int kMinSimtShare = 4;
 constexpr int kTileCost = 2;  // steps that loading a tile's queries and writing its result are worth

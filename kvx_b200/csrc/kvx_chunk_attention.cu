@@ -316,6 +316,7 @@ struct Piece {
   Seq q;
   int32_t seq, head, row0, rows;  // rows [row0, row0 + rows) of the sequence's group rows
   int32_t kv0, kv1;               // K/V tiles of the piece
+  int32_t kv_masked;              // the first K/V tile of which some of the tile's rows may not see every token
   int32_t narrow;
   int32_t slot;                   // partial-result slot, -1 = the piece is the whole tile
 };
@@ -332,6 +333,7 @@ __device__ __forceinline__ Piece piece_of(const ChunkParams &p, const Place &w, 
   const int32_t mul = x.narrow ? 2 : 1;
   x.kv0 = min(n, max(0, w.off - p.tile_cost) * mul);
   x.kv1 = min(n, max(0, end - p.tile_cost) * mul);
+  x.kv_masked = p.causal ? row_limit(p, w.q, x.row0) / p.kv_tile : n;
   // a share holds at most one piece that continues a tile begun earlier and one that begins a
   // tile ended later
   x.slot = (w.off == 0 && end == w.steps) ? -1 : (w.off > 0 ? 2 * share : 2 * share + 1);
@@ -613,6 +615,7 @@ __device__ __forceinline__ float fast_exp2(float x) {  // ex2.approx: 2 ulp, -in
 
 struct Bf16 {
   static constexpr uint32_t kFormat = 1;  // operand format of the instruction descriptor
+  static __device__ __forceinline__ float get(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -624,6 +627,7 @@ struct Bf16 {
 };
 struct Fp16 {
   static constexpr uint32_t kFormat = 0;
+  static __device__ __forceinline__ float get(uint16_t b) { return __half2float(__ushort_as_half(b)); }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 r = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&r);
@@ -710,11 +714,37 @@ __device__ __forceinline__ void stream_range(const ChunkParams &p, const Piece &
   *e = max(x.kv0, min(x.kv1, (limit + kTile - 1) / kTile));
 }
 
+// K/V tiles are taken from the last to the first.  A masked token has weight zero in the products, but
+// zero times an infinity or a NaN that its V holds is a NaN; and tokens that are masked for some of a tile's
+// rows lie in its last tiles only (three at most: the rows of one tile lie within 256 tokens).  So those
+// come first, and behind them, before anything else is added, rows whose sums are not finite get that
+// part again without the masked tokens (repair_rows).  What is not finite later comes from tokens that
+// the row sees, and stays.
+//
+// Of two streams that share their tiles, stream 0 may begin `late` tiles behind stream 1: none of its
+// rows sees those.
+struct Walk {
+  int32_t b, e, late;
+  __device__ __forceinline__ int32_t count() const { return e - b; }
+};
+template <int kStreams>
+__device__ __forceinline__ Walk stream_walk(const ChunkParams &p, const Piece &x, int s) {
+  Walk w;
+  stream_range<kStreams>(p, x, s, &w.b, &w.e);
+  w.late = 0;
+  if (kStreams == 2 && !x.narrow && s == 0) {
+    int b, e;
+    stream_range<kStreams>(p, x, 1, &b, &e);
+    w.late = max(0, e - w.e);
+  }
+  return w;
+}
+
 // The K tiles (and the V tiles) of a piece in the order in which they are consumed: one after the
 // other, or for a narrow piece from the two streams in turn.
 struct TileOrder {
-  int32_t b0, b1, count, narrow;
-  __device__ __forceinline__ int32_t tile(int q) const { return narrow ? ((q & 1) ? b1 : b0) + (q >> 1) : b0 + q; }
+  int32_t e0, e1, count, narrow;
+  __device__ __forceinline__ int32_t tile(int q) const { return narrow ? ((q & 1) ? e1 : e0) - 1 - (q >> 1) : e0 - 1 - q; }
 };
 template <int kStreams>
 __device__ __forceinline__ TileOrder tile_order(const ChunkParams &p, const Piece &x) {
@@ -722,7 +752,7 @@ __device__ __forceinline__ TileOrder tile_order(const ChunkParams &p, const Piec
   stream_range<kStreams>(p, x, 0, &b0, &e0);
   if (kStreams == 2) stream_range<kStreams>(p, x, 1, &b1, &e1);
   const bool narrow = kStreams == 2 && x.narrow;
-  return TileOrder{narrow ? b0 : x.kv0, b1, narrow ? (e0 - b0) + (e1 - b1) : max(e0, e1) - x.kv0, narrow ? 1 : 0};
+  return TileOrder{narrow ? e0 : max(e0, e1), e1, narrow ? (e0 - b0) + (e1 - b1) : max(e0, e1) - x.kv0, narrow ? 1 : 0};
 }
 
 // Whether stream 1 hands its half of a narrow tile to stream 0 (it has K/V tiles of its own).
@@ -1306,22 +1336,19 @@ struct Products {
   }
 
   __device__ __forceinline__ bool piece(const Piece &x) {
-    int n0 = 0, n1 = 0;
+    int late = 0, end[2] = {0, 0};  // places of the streams' tiles: [late, end) and [0, end)
 #pragma unroll
     for (int s = 0; s < S::kStreams; ++s) {
-      int b, e;
-      stream_range<S::kStreams>(p, x, s, &b, &e);
-      const int n = __reduce_max_sync(0xFFFFFFFFu, e - b);  // (uniform, and known to be)
-      if (s == 0)
-        n0 = n;
-      else
-        n1 = n;
+      const Walk w = stream_walk<S::kStreams>(p, x, s);
+      const int n = __reduce_max_sync(0xFFFFFFFFu, w.count());  // (uniform, and known to be)
       if (n == 0) continue;
+      if (s == 0) late = __reduce_max_sync(0xFFFFFFFFu, w.late);
+      end[s] = s == 0 ? late + n : n;
       if (!warp_wait(smem_addr(&m->q_full[s]), q_phase >> s & 1)) return false;
       q_phase ^= 1u << s;
     }
     const bool narrow = S::kStreams == 2 && __any_sync(0xFFFFFFFFu, x.narrow) != 0;
-    const int most = max(n0, n1);
+    const int most = max(end[0], end[1]);
     if (most == 0) return true;
 #pragma unroll 1
     for (int i = 0; i <= most; ++i) {
@@ -1340,13 +1367,13 @@ struct Products {
       bool has_k = false, has_v = false;
 #pragma unroll
       for (uint32_t s = 0; s < 2; ++s) {
-        const int n = s == 0 ? n0 : n1;
-        if (i > 0 && i <= n) {
+        const int from = s == 0 ? late : 0;
+        if (i > from && i <= end[s]) {
           if (!has_v && !acquire(v_ring)) return false;
           has_v = true;
-          if (!output(s, i == 1, i == n)) return false;
+          if (!output(s, i - 1 == from, i == end[s])) return false;
         }
-        if (i < n) {
+        if (i >= from && i < end[s]) {
           if (!has_k && !acquire(k_ring)) return false;
           has_k = true;
           scores(s);
@@ -1392,38 +1419,107 @@ __device__ __forceinline__ bool pages_exist(const ChunkParams &p, const Piece &x
   return tok >= x.q.len || ((p.block_size & 3) == 0 && page_of(p, x.seq, tok) >= 0);
 }
 
-// One row of a piece again, token by token and only those it may see, under the maximum `mx` its
-// weights were made with.  A masked token has weight zero in the products, but zero times an
-// infinity or a NaN that its V holds is a NaN: a row that comes out of the products not finite
-// although tokens were masked for it is redone here.
+// Whether one of this row's sums is not finite.
 template <int kDp>
-__device__ __noinline__ void redo_row(const ChunkParams &p, const Piece &x, int32_t r, float mul, float mx, float *o) {
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = kDp / 32;
+__device__ __forceinline__ bool sums_not_finite(uint32_t o_at) {
+  const float2 zero = make_float2(0.f, 0.f);
+  float2 f0 = zero, f1 = zero;  // become NaN with the first value that is not finite
+#pragma unroll 1
+  for (int k = 0; k < kDp; k += 64) {
+    float a[32], b[32];
+    tc_ld32(a, o_at + k);
+    tc_ld32(b, o_at + k + 32);
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      f0 = __ffma2_rn(make_float2(a[i], a[i + 1]), zero, f0);
+      f1 = __ffma2_rn(make_float2(b[i], b[i + 1]), zero, f1);
+    }
+  }
+  return (f0.x + f0.y) + (f1.x + f1.y) != 0.f;
+}
+
+// The sums of the rows of a warp that are `bad` once more, over the tokens [first, limit) that the row sees,
+// with the weights they were made with (exp2(mul * score + sub)).  A few tokens at a time, every lane its own
+// row: all lanes read the same elements of K and V.  At most three tiles of tokens, about 4 ms at head_dim 128, far
+// below what the other roles' waits allow: a prompt of 8 000 tokens x 8 heads with no finite value in V takes
+// 8.8 ms (9.9 from packed pages, 22 at head_dim 256).  Looking for such rows costs the 16 prompts of the note
+// at the kernel 1 %, the order of the tiles 2 % (4 x 512 tokens over 32k gain 3 % by it).
+template <typename T, int kDp, bool kFp8>
+__device__ __noinline__ void repair_rows(const ChunkParams &p, const Piece &x, bool bad, int32_t r, int32_t first, int32_t limit, float mul,
+                                         float sub, uint32_t o_at) {
+  constexpr int kTok = 8;
+  auto q_at = [](const char *at) { return T::get(*reinterpret_cast<const uint16_t *>(at)); };
+  auto kv_at = [&](const char *at) { return kFp8 ? load_f32(at, KVX_DTYPE_F8_E4M3) : q_at(at); };
+  if (!bad) r = x.row0, limit = 0;
   const int32_t token = r / p.group, qh = x.head * p.group + r % p.group;
   const char *q = p.query + (x.q.first + token) * p.q_pitch + static_cast<int64_t>(qh) * p.dim * 2;
-  const float sub = mx == -INFINITY ? 0.f : -mx * fabsf(mul);
+  const int32_t end = __reduce_max_sync(0xFFFFFFFFu, limit);
 #pragma unroll 1
-  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  const int32_t end = min(row_limit(p, x.q, r), x.kv1 * kTile);
-#pragma unroll 1
-  for (int32_t t = x.kv0 * kTile; t < end; ++t) {
-    const int32_t page = page_of(p, x.seq, t);
-    if (page < 0) continue;
-    const int32_t at = t % p.block_size;
-    const char *kp = p.k.base + page * p.k.blk, *vp = p.v.base + page * p.v.blk;
-    float dot = 0.f;
-#pragma unroll 1
-    for (int d = lane; d < p.dim; d += 32)
-      dot = fmaf(load_f32(q + d * 2, p.io_code), load_f32(kp + head_offset(p.k, at, x.head, d), p.cache_code), dot);
+  for (int k = 0; k < kDp; k += 16) {
+    float o[16];
+    tc_ld16(o, o_at + k);
+    tc_wait_ld();
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, s);
-    const float w = exp2f(fmaf(dot, mul, sub));
+    for (int i = 0; i < 16; ++i) o[i] = bad ? 0.f : o[i];
+    tc_st16(o_at + k, reinterpret_cast<const uint32_t *>(o));
+  }
+  tc_wait_st();
+  if (p.num_blocks == 0) return;
 #pragma unroll 1
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 32 * i;
-      if (d < p.dim) o[i] = fmaf(w, load_f32(vp + head_offset(p.v, at, x.head, d), p.cache_code), o[i]);
+  for (int32_t t0 = first; t0 < end; t0 += kTok) {
+    const char *at[kTok];  // K, then V; of page 0 for tokens that are left out
+    float w[kTok];
+    uint32_t in = 0;
+    auto rows = [&](const PageView &v) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        const int32_t t = t0 + i, page = t < end ? page_of(p, x.seq, t) : -1;
+        at[i] = v.base + max(page, 0) * v.blk + static_cast<int64_t>(t % p.block_size) * v.tok + x.head * v.head;
+        if (page >= 0 && t < limit) in |= 1u << i;
+      }
+    };
+    // from one element to the next
+    int32_t left;
+    auto step = [&](const PageView &v) {
+      int64_t by = v.dlo;
+      if (--left == 0) by = v.dhi - (v.pack - 1) * v.dlo, left = v.pack;
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) at[i] += by;
+    };
+    rows(p.k);
+    left = p.k.pack;
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) w[i] = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < p.dim; ++d) {
+      const float y = q_at(q + d * 2);
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) w[i] = fmaf(y, kv_at(at[i]), w[i]);
+      step(p.k);
     }
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) w[i] = exp2f(fmaf(w[i], mul, sub));
+    rows(p.v);
+    left = p.v.pack;
+#pragma unroll 1
+    for (int k = 0; k < p.dim; k += 16) {
+      float o[16];
+      tc_ld16(o, o_at + k);
+      tc_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        if (k + c >= p.dim) continue;
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+          const float v = kv_at(at[i]);
+          o[c] = (in >> i) & 1 ? fmaf(w[i], v, o[c]) : o[c];
+        }
+        step(p.v);
+      }
+      tc_st16(o_at + k, reinterpret_cast<const uint32_t *>(o));
+    }
+    tc_wait_st();
   }
 }
 
@@ -1483,9 +1579,9 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
     }
     const bool narrow = S::kStreams == 2 && x.narrow;
     const int count = narrow ? e - b + other : max(e - b, other);  // tiles of the piece, each of K and of V
-    // this stream is the last reader of its tile i (stream 1 comes after stream 0)
-    auto last_reader = [&](int i) { return narrow || s == 1 || i >= other; };
-    auto place = [&](int i) { return narrow ? 2 * i + s : i; };
+    // this stream is the last reader of its tiles (stream 1 comes after stream 0, and takes every tile)
+    const bool last_reader = narrow || s == 1 || other == 0;
+    auto place = [&](int i) { return narrow ? 2 * i + s : i; };  // of this stream's tile i, where it is the last reader
     const int32_t row_at = x.row0 + (narrow ? 0 : s * kTile);   // first group row of this stream
     const int32_t rows = min(kTile, x.rows - (narrow ? 0 : s * kTile));
     if (rows <= 0) {
@@ -1536,15 +1632,15 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
     const int32_t limit = tid < rows ? row_limit(p, x.q, row_at + tid) : INT32_MAX;
     float mx = -INFINITY, l = 0.f;
     const uint32_t o_at = tmem0 + lanes + 256 + s * kDp;
-    int from = b;
+    int from = e;
     if ((tid & ~31) >= rows) {
       // All rows of this warp lie behind the tile's last: no weights to make.  What the products do
       // with its lanes stays in its lanes.
 #pragma unroll 1
-      for (; from < e; ++from, ++tiles) {
+      for (; from > b; --from, ++tiles) {
         const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
         if (!warp_wait(smem_addr(&m->s_full[0]) + 8 * buf, (S::kScoreBufs == 2 ? tiles >> 1 : tiles) & 1)) return;
-        if (S::kStreams == 1 && from > b && !warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
+        if (S::kStreams == 1 && from < e && !warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
         if (lane == 0) {
           mbar_arrive(smem_addr(&m->p_part[0]) + 8 * buf);
           mbar_arrive(smem_addr(&m->p_full[0]) + 8 * buf);
@@ -1552,9 +1648,23 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
         __syncwarp();
       }
     }
-    bool page_ok = pages_exist(p, x, b * kTile);
+    // Called when all products so far have ended, and only tiles with masked tokens are among them: [masked, e).
+    const int masked = max(b, min(e, x.kv_masked));
+    const bool any_masked = __any_sync(0xFFFFFFFFu, limit < min(x.q.len, e * kTile)) != 0 && masked < e;
+    auto repair = [&]() {
+      const bool bad = sums_not_finite<kDp>(o_at) && limit < min(x.q.len, e * kTile);
+      if (!__any_sync(0xFFFFFFFFu, bad)) return;
+      const Piece y = x;  // (a copy: the reference keeps it in memory)
+      const float sub = mx == -INFINITY ? 0.f : -mx * am;
+      if (p.cache_code == KVX_DTYPE_F8_E4M3)
+        repair_rows<T, kDp, true>(p, y, bad, row_at + tid, masked * kTile, limit, mul, sub, o_at);
+      else
+        repair_rows<T, kDp, false>(p, y, bad, row_at + tid, masked * kTile, limit, mul, sub, o_at);
+    };
+    const int repair_at = any_masked ? masked - 1 : -1;  // the tile ahead of which that is
+    bool page_ok = pages_exist(p, x, max(e - 1, 0) * kTile);
 #pragma unroll 1
-    for (int j = from; j < e; ++j, ++tiles) {
+    for (int j = from - 1; j >= b; --j, ++tiles) {
       const uint32_t buf = S::kScoreBufs == 2 ? (tiles & 1) : s;
       const uint32_t ph = (S::kScoreBufs == 2 ? tiles >> 1 : tiles) & 1;
       const uint32_t s_at = tmem0 + lanes + buf * kTile;
@@ -1564,10 +1674,15 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
       if (!warp_wait(smem_addr(&m->s_full[0]) + 8 * buf, ph)) return;
       tc_fence_after();
       // these scores have read their K tile, and (two streams) the product ahead of them its V tile
-      const int i = j - b;
-      if (last_reader(i)) release(0, place(i));
-      if (S::kStreams == 2 && i > 0 && last_reader(i - 1)) release(1, place(i - 1));
-      if (j == e - 1 && p.q_tma && tid == 0 && !(s == 1 && joins_streams(x))) mbar_arrive(smem_addr(&m->q_empty[0]) + 8 * s);
+      const int i = e - 1 - j;
+      if (last_reader) release(0, place(i));
+      if (S::kStreams == 2 && i > 0 && last_reader) release(1, place(i - 1));
+      if (j == b && p.q_tma && tid == 0 && !(s == 1 && joins_streams(x))) mbar_arrive(smem_addr(&m->q_empty[0]) + 8 * s);
+      if (j == repair_at) {
+        if (S::kStreams == 1 && !warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
+        tc_fence_after();
+        repair();
+      }
       if (!plain) correct_scores(p, x, s_at, j * kTile, valid, gaps, sign);
       float top = -INFINITY;
 #pragma unroll 1
@@ -1586,12 +1701,12 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
         }
         top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
       }
-      page_ok = pages_exist(p, x, (j + 1) * kTile);  // of the next tile: on its way meanwhile
+      page_ok = pages_exist(p, x, max(j - 1, 0) * kTile);  // of the next tile: on its way meanwhile
       const bool raise = top > mx && (mx == -INFINITY || (top - mx) * am > kLazy);
       if (__any_sync(0xFFFFFFFFu, raise)) {
         const float c = raise ? weight_of(mx, top, am) : 1.f;
         if (raise) mx = top;
-        if (j > b) {
+        if (j < e - 1) {
           l *= c;
           // the sums of the tiles so far must be complete before they are rescaled (two streams: they
           // are, these scores were announced behind them)
@@ -1630,7 +1745,7 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
             // previous output product, so they do not tell that it has ended.  Weights are handed over
             // only after it has -- its barrier is then never more than one phase away from the
             // parity that is waited for.
-            if (S::kStreams == 1 && j > b) {
+            if (S::kStreams == 1 && j < e - 1) {
               if (!warp_wait(smem_addr(&m->pv_done[0]), (tiles - 1) & 1)) return;
               release(1, i - 1);
             }
@@ -1654,7 +1769,8 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
       if (!warp_wait(smem_addr(&m->pv_done[0]) + 8 * s, (S::kStreams == 1 ? tiles - 1 : pieces) & 1)) return;
       tc_fence_after();
       ++pieces;
-      if (last_reader(e - b - 1)) release(1, place(e - b - 1));
+      if (last_reader) release(1, place(e - b - 1));
+      if (masked == b && any_masked) repair();  // no other tiles came behind those with masked tokens
     }
     entries += count;
     const float vmul = p.vs.base != nullptr ? p.vs.base[x.head * p.vs.stride] : 1.f;
@@ -1702,7 +1818,6 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
     char *out = p.out + (x.q.first + token) * p.o_pitch + static_cast<int64_t>(qh) * p.dim * 2;
     const int64_t part = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + (r - x.row0);
     const float mul_out = l == 0.f ? 0.f : (x.slot < 0 ? vmul / l : vmul);
-    float finite = 0.f;  // becomes NaN with the first value that is not finite
     const bool vec_out = p.q_vec != 0;
     char *quad_out[4];  // the rows of this thread and its three neighbours
 #pragma unroll
@@ -1729,10 +1844,7 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
         for (int i = 0; i < 32; ++i) o[i] = o[i] * f_own + joint[(k % (kDp / 2) + i) * kTile] * f_other;
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        o[i] = l == 0.f ? 0.f : o[i] * mul_out;
-        finite = fmaf(o[i], 0.f, finite);
-      }
+      for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * mul_out;
       if (x.slot < 0 && vec_out) {
         // A thread has 64 bytes of its row; four threads exchange 16-byte pieces so that each store
         // instruction writes 64 bytes of 8 rows instead of 16 bytes of 32.
@@ -1790,29 +1902,6 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
     }
     if (x.slot >= 0 && tid < rows) reinterpret_cast<float2 *>(p.part_ml)[part] = make_float2(mx, l);
     tc_fence_before();
-    const int32_t seen = min(x.q.len, x.kv1 * kTile);
-    unsigned again = __ballot_sync(0xFFFFFFFFu, tid < rows && finite != 0.f && limit < seen);
-    while (again != 0) {
-      const int from = __ffs(again) - 1;
-      again &= again - 1;
-      const int32_t rr = row_at + (tid & ~31) + from;
-      float o[kDp / 32];
-      const Piece y = x;  // (a copy: the reference keeps it in memory)
-      redo_row<kDp>(p, y, rr, mul, __shfl_sync(0xFFFFFFFFu, mx, from), o);
-      const float f = __shfl_sync(0xFFFFFFFFu, mul_out, from);
-      const int32_t tk = rr / p.group, hh = x.head * p.group + rr % p.group;
-      char *to = p.out + (x.q.first + tk) * p.o_pitch + static_cast<int64_t>(hh) * p.dim * 2;
-      const int64_t slot_row = x.slot < 0 ? 0 : static_cast<int64_t>(x.slot) * p.slot_rows + (rr - x.row0);
-#pragma unroll 1
-      for (int i = 0; i < kDp / 32; ++i) {
-        const int d = lane + 32 * i;
-        if (d >= p.dim) continue;
-        if (x.slot >= 0)
-          p.part_o[slot_row * p.dim + d] = o[i] * f;
-        else
-          store_f32(to, d, o[i] * f, p.io_code);
-      }
-    }
   }
 }
 

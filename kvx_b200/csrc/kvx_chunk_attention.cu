@@ -615,6 +615,7 @@ __device__ __forceinline__ float fast_exp2(float x) {  // ex2.approx: 2 ulp, -in
 
 struct Bf16 {
   static constexpr uint32_t kFormat = 1;  // operand format of the instruction descriptor
+  static constexpr float kShift = 0.f;    // of the softmax weights, see kLazy; bf16 has the exponents of f32
   static __device__ __forceinline__ float get(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
@@ -627,6 +628,7 @@ struct Bf16 {
 };
 struct Fp16 {
   static constexpr uint32_t kFormat = 0;
+  static constexpr float kShift = 7.f;
   static __device__ __forceinline__ float get(uint16_t b) { return __half2float(__ushort_as_half(b)); }
   static __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __half2 r = __floats2half2_rn(lo, hi);
@@ -1392,8 +1394,10 @@ struct Products {
 // ---- softmax ------------------------------------------------------------------------------
 
 // Raises the weights' reference maximum only when it has moved by more than this (in the exp2
-// domain): weights then stay below 2^8, the rounding of a weight is relative either way, and the
-// sums in tensor memory are rescaled on a few tiles instead of on every one.
+// domain): weights then stay below 2^8, and the sums in tensor memory are rescaled on a few tiles instead
+// of on every one.  Weights, and with them their sums, are carried as 2^kShift times themselves: below
+// 2^15 in f16 (whose largest value is 65504), where the rounding of a weight is relative down to 2^-21 and at most
+// 2^-32 below that, so that a long context of little weight beside one dominant token is not lost.
 constexpr float kLazy = 8.f;
 
 // Weights of 32 scores of one row: exponentials, their sum, and the rounded pairs to tensor memory.
@@ -1655,7 +1659,7 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
       const bool bad = sums_not_finite<kDp>(o_at) && limit < min(x.q.len, e * kTile);
       if (!__any_sync(0xFFFFFFFFu, bad)) return;
       const Piece y = x;  // (a copy: the reference keeps it in memory)
-      const float sub = mx == -INFINITY ? 0.f : -mx * am;
+      const float sub = mx == -INFINITY ? T::kShift : fmaf(-mx, am, T::kShift);
       if (p.cache_code == KVX_DTYPE_F8_E4M3)
         repair_rows<T, kDp, true>(p, y, bad, row_at + tid, masked * kTile, limit, mul, sub, o_at);
       else
@@ -1723,8 +1727,8 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
           }
         }
       }
-      // weights exp2((score - mx) * am); a row that has seen no token yet subtracts 0
-      const float sub = mx == -INFINITY ? 0.f : -mx * am;
+      // weights exp2((score - mx) * am + kShift); a row that has seen no token yet subtracts 0
+      const float sub = mx == -INFINITY ? T::kShift : fmaf(-mx, am, T::kShift);
       const float2 mul2 = make_float2(am, am), sub2 = make_float2(sub, sub);
       float2 sum2 = make_float2(0.f, 0.f);
       {

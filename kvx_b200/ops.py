@@ -419,7 +419,7 @@ def attention_workspace_bytes(seq_count: int, q_heads: int, kv_heads: int, dim: 
 
 
 def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none", scale: float = 1.0,
-                    original_length: int = 8192, low: float = 1.0, high: float = 4.0,
+                    original_length: int = 8192, low: float = 1.0, high: Optional[float] = None,
                     device: Optional[torch.device] = None) -> tuple[torch.Tensor, float]:
     """``(inv_freq, factor)`` for :func:`rotary_embedding`: float64 radians per position of the
     ``rotary_dim / 2`` pairs, and the factor on the turned values.
@@ -429,7 +429,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none
     the slowest pair is divided by ``scale`` and the fastest kept; ``"bands"``, pairs that turn more
     than ``high`` times over the original length kept, fewer than ``low`` times divided, linear in
     the turns in between; ``"ramp"``, the same decision linear in the pair's index between the pairs
-    that turn ``high`` and ``low`` times, with the factor ``0.1 ln(scale) + 1``."""
+    that turn ``high`` and ``low`` times, with the factor ``0.1 ln(scale) + 1``.  ``high`` is 4 for
+    ``"bands"`` and 32 for ``"ramp"`` unless given."""
     if rotary_dim <= 0 or rotary_dim % 2 != 0:
         raise ValueError("rotary_dim must be positive and even")
     if not scale > 0 or not base > 1:
@@ -444,6 +445,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none
     if scaling == "linear":
         freq = freq / scale
     elif scaling in ("bands", "ramp"):
+        if high is None:
+            high = 4.0 if scaling == "bands" else 32.0
         if not high > low > 0:
             raise ValueError("high and low must be turns with high > low > 0")
         if scaling == "bands":

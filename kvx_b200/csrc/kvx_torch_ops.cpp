@@ -448,11 +448,12 @@ void rotary_and_cache(const torch::Tensor &query, const torch::Tensor &key, cons
                                  &slot_mapping, static_cast<const torch::Tensor *>(&query_out)})
     TORCH_CHECK(t->device() == query.device(), "all tensors must be on the query's device");
   const kvx_dtype_t slot_dtype = index_code(slot_mapping.scalar_type());
-  TORCH_CHECK(slot_dtype != KVX_DTYPE_INVALID && slot_mapping.dim() == 1 && slot_mapping.is_contiguous() &&
-                  slot_mapping.numel() == key.size(0),
-              "slot_mapping must hold one int32 or int64 slot per token");
+  TORCH_CHECK(slot_dtype != KVX_DTYPE_INVALID && slot_mapping.dim() == 1 && slot_mapping.is_contiguous(),
+              "slot_mapping must be a contiguous int32 or int64 vector");
+  // rows behind the last slot (a batch padded to a fixed size) are turned, but not cached
+  const int64_t tokens = slot_mapping.numel(), rows = key.size(0), heads = key.size(1), dim = key.size(2);
+  TORCH_CHECK(tokens <= rows, "key/value hold fewer tokens than slot_mapping");
   const at::cuda::OptionalCUDAGuard guard(at::device_of(query));
-  const int64_t tokens = key.size(0), heads = key.size(1), dim = key.size(2);
   kvx_cache_desc_t cache;
   describe_cache(&cache, key_cache, value_cache, kv_cache_dtype, heads, dim);
   kvx_write_desc_t write;
@@ -464,6 +465,7 @@ void rotary_and_cache(const torch::Tensor &query, const torch::Tensor &key, cons
   write.io.head_dim = static_cast<uint32_t>(dim);
   describe(&write.io.key, key, io, KVX_LAYOUT_INVALID);
   describe(&write.io.value, value, io, KVX_LAYOUT_INVALID);
+  write.io.key.shape[0] = write.io.value.shape[0] = tokens;
   write.slots.size = sizeof(write.slots);
   write.slots.dtype = slot_dtype;
   write.slots.token_count = static_cast<uint32_t>(tokens);
@@ -472,13 +474,22 @@ void rotary_and_cache(const torch::Tensor &query, const torch::Tensor &key, cons
   describe_scale(&write.k_scale_desc, k_scale, heads);
   describe_scale(&write.v_scale_desc, v_scale, heads);
   kvx_rotary_desc_t r;
-  describe_rotary(&r, positions, inv_freq, interleaved, factor, false, tokens, query.device());
+  describe_rotary(&r, positions, inv_freq, interleaved, factor, false, rows, query.device());
   if (query.numel() > 0) {
     describe(&r.query, query, io, KVX_LAYOUT_INVALID);
     describe(&r.query_out, query_out, io, KVX_LAYOUT_INVALID);
+    r.query.shape[0] = r.query_out.shape[0] = tokens;
   }
-  const kvx_status_t status = kvx_launch_rotary_write_kv(&cache, &write, &r, current_stream());
+  kvx_status_t status = kvx_launch_rotary_write_kv(&cache, &write, &r, current_stream());
   TORCH_CHECK(status == KVX_STATUS_OK, "kvx rotary write failed with status=", static_cast<int>(status));
+  if (tokens == rows || query.numel() == 0) return;
+  const torch::Tensor rest = query.narrow(0, tokens, rows - tokens), rest_out = query_out.narrow(0, tokens, rows - tokens),
+                      rest_at = positions.narrow(0, tokens, rows - tokens);
+  describe_rotary(&r, rest_at, inv_freq, interleaved, factor, false, rows - tokens, query.device());
+  describe(&r.query, rest, io, KVX_LAYOUT_INVALID);
+  describe(&r.query_out, rest_out, io, KVX_LAYOUT_INVALID);
+  status = kvx_launch_rotary(&r, current_stream());
+  TORCH_CHECK(status == KVX_STATUS_OK, "kvx rotary failed with status=", static_cast<int>(status));
 }
 
 // Page upkeep (include/kvx_pages_ops.h).  Whole pages are moved, so a 4-D tensor is described with

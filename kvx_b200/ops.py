@@ -533,7 +533,8 @@ def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     """:func:`rotary_embedding` of ``query`` and ``key`` and :func:`reshape_and_cache_flash_kvx` of the
     turned keys and of ``value`` in one pass: the pages hold the same bits, ``key`` stays as it is.
     Returns ``query_out`` (new unless given; ``query`` itself turns in place).  Tokens with a negative
-    slot are turned but not cached."""
+    slot, and those behind the last slot of a shorter ``slot_mapping`` (a batch padded to a fixed
+    size), are turned but not cached."""
     if query_out is None:
         query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     native = native_ops() if key_cache.dim() == 4 and query.is_cuda else None
@@ -549,14 +550,15 @@ def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         raise ValueError("query must match key in dtype, tokens and dim")
     if query_out.shape != query.shape or query_out.dtype != query.dtype:
         raise ValueError("query_out must match query")
-    if slot_mapping.dtype not in _INDEX_CODES or slot_mapping.dim() != 1 or slot_mapping.numel() != key.shape[0] \
+    if slot_mapping.dtype not in _INDEX_CODES or slot_mapping.dim() != 1 or slot_mapping.numel() > key.shape[0] \
             or not slot_mapping.is_contiguous():
-        raise ValueError("slot_mapping must hold one int32 or int64 slot per token")
+        raise ValueError("slot_mapping must be a contiguous int32 or int64 vector, one slot per token at most")
     for name, t in (("key", key), ("value", value), ("key_cache", key_cache), ("value_cache", value_cache),
                     ("slot_mapping", slot_mapping), ("query_out", query_out)):
         if not t.is_cuda or t.device != query.device:
             raise ValueError(f"{name} must be on the query's CUDA device")
-    tokens, heads, dim = key.shape
+    rows, heads, dim = key.shape
+    tokens = slot_mapping.numel()
     cache = cache_desc_from_tensors(key_cache, value_cache, kv_cache_dtype, heads)
     w = abi.write_desc(tokens, heads, dim, _FLOAT_CODES[key.dtype], key.data_ptr(), value.data_ptr(),
                        _INDEX_CODES[slot_mapping.dtype], slot_mapping.data_ptr(), k_scale=_scale_desc(k_scale, heads),
@@ -565,12 +567,15 @@ def rotary_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         for i, s in enumerate(src.stride()):
             t.stride[i] = s
     some = query.numel() > 0
-    r = _rotary_desc(query if some else None, query_out if some else None, tokens, query.device, positions, inv_freq,
+    r = _rotary_desc(query if some else None, query_out if some else None, rows, query.device, positions, inv_freq,
                      interleaved, factor, False)
+    r.query.shape[0] = r.query_out.shape[0] = tokens
     with torch.cuda.device(query.device):
         status = lib().kvx_launch_rotary_write_kv(C.byref(cache), C.byref(w), C.byref(r), _stream())
     if status != abi.STATUS_OK:
         raise KvxError("kvx rotary write", status)
+    if tokens < rows and some:
+        rotary_embedding(query[tokens:], None, positions[tokens:], inv_freq, interleaved, factor, query_out=query_out[tokens:])
     return query_out
 
 

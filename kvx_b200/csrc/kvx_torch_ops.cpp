@@ -329,7 +329,7 @@ void describe_lens(kvx_seq_lens_t *d, const torch::Tensor &t, const torch::Tenso
 }
 
 // Attention of a chunk of new tokens (include/kvx_attention.h).  An empty or short `workspace` is
-// replaced by scratch of torch's allocator.
+// replaced by scratch of torch's allocator; max_seq_len = 0 stands for what the table can address.
 void paged_attention_chunk(torch::Tensor &out, const torch::Tensor &query, const torch::Tensor &key_cache,
                            const torch::Tensor &value_cache, const torch::Tensor &block_table, const torch::Tensor &seq_lens,
                            const torch::Tensor &query_indptr, double scale, bool causal, int64_t max_seq_len,
@@ -360,7 +360,8 @@ void paged_attention_chunk(torch::Tensor &out, const torch::Tensor &query, const
                                : key_cache.size(1);
   kvx_cache_desc_t cache;
   describe_cache(&cache, key_cache, value_cache, kv_cache_dtype, kv_heads, dim);
-  if (max_seq_len <= 0)
+  TORCH_CHECK(max_seq_len >= 0, "max_seq_len must not be negative");
+  if (max_seq_len == 0)
     max_seq_len = std::min<int64_t>(block_table.size(1) * static_cast<int64_t>(cache.block_size), INT32_MAX - 2048);
   TORCH_CHECK(max_seq_len <= INT32_MAX - 1024, "max_seq_len is too large");
   a.size = sizeof(a);

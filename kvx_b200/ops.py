@@ -367,6 +367,8 @@ def paged_attention_chunk(query: torch.Tensor, key_cache: torch.Tensor, value_ca
     if query_indptr.dtype not in _INDEX_CODES or query_indptr.dim() != 1 or query_indptr.numel() != seqs + 1 \
             or not query_indptr.is_contiguous():
         raise ValueError("query_indptr must hold seq_count + 1 int32 or int64 row numbers")
+    if max_seq_len is not None and max_seq_len < 1:
+        raise ValueError("max_seq_len must be positive")
     rows, q_heads, dim = query.shape
     if out is None:
         out = torch.empty((rows, q_heads, dim), dtype=query.dtype, device=query.device)

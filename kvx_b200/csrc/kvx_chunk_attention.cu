@@ -68,6 +68,7 @@ struct ChunkParams {
   int32_t q_tma;               // 1: query tiles are loaded by TMA
   int32_t q_vec;               // 1: query rows can be read, out rows written in 16-byte pieces
   int32_t kv_vec;              // 1: page rows can be read in 16-byte pieces
+  int32_t test_stall;          // 1: the first CTA's schedule waits for something that never comes, see the kernel
 };
 
 __device__ int g_chunk_error;  // set to 1 when a bounded wait gave up
@@ -479,10 +480,11 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits for the phase, at most two seconds (kTries suspensions of up to a microsecond); a wait that
-// gives up sets the device's word and answers false, upon which its role returns.  Few
-// instructions on purpose, see the note at the kernel.
-constexpr uint32_t kTries = 2000000;
+// Waits for the phase, two seconds at most; a wait that gives up sets the device's word and answers false,
+// upon which its role returns.  Few instructions on purpose, see the note at the kernel: tries are
+// counted, not time.  A try that fails takes 4.0 us on B200 (measured over 1 to 100 000 of them, with one warp of
+// the CTA waiting and with twelve), whatever the suspension asked for.
+constexpr uint32_t kTries = 500000;
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -1973,6 +1975,9 @@ __global__ void __launch_bounds__(kLoads == kTmaLoads ? 384 : 512, 1)  // = thre
 
   if (warp < kMmaWarp) {
     if (S::kStreams == 2 || warp < 4) softmax_role<T, kDp>(p, base, smem, tmem, m);
+  } else if (p.test_stall != 0 && blockIdx.x == 0 && warp == kMmaWarp + 1 && !warp_wait(smem_addr(&m->tail), 0)) {
+    // A test of the bounded waits: the warp that publishes the pieces gives up before it has published or loaded
+    // anything, the others when no piece comes.
   } else {
     if (warp == kMmaWarp) {
       Products<T, kDp> pr(p, base, __reduce_max_sync(0xFFFFFFFFu, tmem), m);
@@ -2694,6 +2699,7 @@ KVX_API kvx_status_t kvx_launch_paged_attention_chunk(const kvx_cache_desc_t *ca
   p.kv_tile = sp.kv_tile;
   p.tile_cost = sp.tile_cost;
   p.pair = tensor && D <= 128 ? 1 : 0;
+  p.test_stall = kvx_b200_get_option("chunk_test_stall") != 0 ? 1 : 0;
   p.q_vec = D % 8 == 0 && p.q_pitch % 16 == 0 && p.o_pitch % 16 == 0 && aligned16(p.query) && aligned16(p.out) ? 1 : 0;
   const cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
 

@@ -83,6 +83,7 @@ struct Options {
   std::atomic<int64_t> packed_tiles{1};           // 1 = transposing tile kernels for HND_PACKED pages where they apply
   std::atomic<int64_t> bulk_wait_us{1000000};     // a bulk-path wait on a copy is abandoned after this long
   std::atomic<int64_t> bulk_test_stall{0};        // test hook: pipe 0 of CTA 0 first waits on a barrier nothing completes
+  std::atomic<int64_t> chunk_test_stall{0};       // test hook: the same for the schedule of CTA 0 of the chunk attention
 };
 Options g_opt;
 inline int64_t opt(const std::atomic<int64_t> &knob) { return knob.load(std::memory_order_relaxed); }
@@ -93,6 +94,7 @@ struct OptionName {
   std::atomic<int64_t> Options::*field;
 };
 const OptionName kOptionNames[] = {
+    {"chunk_test_stall", &Options::chunk_test_stall},
     {"write_vecs_per_cta", &Options::write_vecs_per_cta},
     {"write_unroll", &Options::write_unroll},
     {"gather_path", &Options::gather_path},

@@ -89,8 +89,9 @@ KVX_API kvx_status_t kvx_launch_paged_attention_decode(const kvx_cache_desc_t *c
  * read after others were written).  Scores, softmax and sums are f32; on the tensor-core path the
  * softmax weights are rounded once to the query's type before they multiply V: a relative error of
  * half a unit in the last place of that type, of the order of the output's own rounding, and in f16
- * for weights below 2^-21 of the row's largest an absolute one of at most 2^-32 of it.  The result is
- * rounded once to the query's type. */
+ * for weights below 2^-21 of the row's largest an absolute one of at most 2^-32 of it (an infinity in
+ * the V of a token whose weight becomes zero gives NaN).  The result is rounded once to the query's
+ * type. */
 typedef struct kvx_chunk_attention_desc {
   uint32_t size;
   uint32_t num_q_heads;    /* a multiple of cache->num_kv_heads */

@@ -1914,14 +1914,16 @@ __device__ __forceinline__ void softmax_role(const ChunkParams &p, uint32_t base
 // Every role's instruction count is part of the kernel's speed: a single warp gets through about one
 // instruction in eight clocks here, so loops over columns are kept as loops of 32 to 64 columns that
 // fit the registers, and what is done per tile by the loading and the issuing warps is kept small.
-// Measured on 16 prompts of 512 to 4096 tokens and on 4 x 512 tokens over 32k contexts (us):
+// Measured on 16 prompts of 512 to 4096 tokens and on 4 x 512 tokens over 32k contexts (us), in runs too short to
+// reach the power cap:
 //   first version, one thread issuing everything, boxes issued by their lanes     2410   1310
 //   queries by TMA, column loops, waits that do not read the timer first          1290   1110 - 1250
 //   + whole boxes, two loading warps, converged issue, one commit per product     1180   1080 - 1220
-// (824 and 950 TFLOP/s; behind other work, at the power cap, 1350 and 1250.)  64 x 5 drafted tokens over up to
-// 32k, bound by the loads: 226, 4.7 TB/s.  Two warps per 32 rows (half the columns each, 640 threads) ran
-// at 1470 and 1340; keeping all 128 scores of a row in registers at 1490 and 1390, the column loops
-// unrolled at 1440 and 1230; strict turns between the streams changed nothing.
+// Back to back, at the cap, and with the tiles from the last to the first: 1390 and 1210 (700 and 850 TFLOP/s).
+// 64 x 5 drafted tokens over up to 32k, bound by the loads: 245, 4.3 TB/s.  Two warps per 32 rows (half the
+// columns each, 640 threads) ran at 1470 and 1340 against 1350 and 1250 then; keeping all 128 scores of a row in
+// registers at 1490 and 1390, the column loops unrolled at 1440 and 1230; strict turns between the
+// streams changed nothing.
 template <typename T, int kDp, Loads kLoads>
 __global__ void __launch_bounds__(kLoads == kTmaLoads ? 384 : 512, 1)  // = threads_of(kLoads)
     kvx_chunk_attention_kernel(const __grid_constant__ ChunkParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
